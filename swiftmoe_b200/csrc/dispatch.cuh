@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(256) combine_warp_kernel(const T* __restrict__
   for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < T_; t += warps) {
     const int my_r = lane < k ? slot_row[t * k + lane] : -1;
     const float my_w = lane < k ? w[t * k + lane] : 0.f;
-    for (int c0 = lane; c0 < nv; c0 += 32 * U) {
+    for (int c0 = lane; c0 - lane < nv; c0 += 32 * U) {
       float acc[U][VEC];
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(256) permute_tokens_kernel(const unsigned char
     const unsigned live = __ballot_sync(0xffffffffu, my_r >= 0);
     if (live == 0) continue;
     const uint4* src = reinterpret_cast<const uint4*>(x + t * row_bytes);
-    for (int c0 = lane; c0 < nv; c0 += 32 * U) {
+    for (int c0 = lane; c0 - lane < nv; c0 += 32 * U) {
       uint4 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) v[u] = c0 + u * 32 < nv ? src[c0 + u * 32] : make_uint4(0u, 0u, 0u, 0u);
