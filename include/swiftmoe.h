@@ -52,6 +52,16 @@ typedef struct CUstream_st* smoe_stream_t; /* == cudaStream_t */
 #define SMOE_EXPERT_LINEAR 0 /* y = x W_e^T           (one bias-free d x d linear)      */
 #define SMOE_EXPERT_SWIGLU 1 /* y = w2(silu(w1 x) * w3 x)                               */
 
+/* ------------------------------------------------- activations of smoe_grouped_linear */
+#define SMOE_ACT_NONE 0
+#define SMOE_ACT_RELU 1
+#define SMOE_ACT_GELU 2      /* z Phi(z)                                                 */
+#define SMOE_ACT_GELU_TANH 3 /* z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))            */
+#define SMOE_ACT_SILU 4      /* z / (1 + e^-z)                                           */
+/* layouts of smoe_grouped_linear's weights */
+#define SMOE_W_NK 0 /* [G, N, K], nn.Linear's: C = A W_g^T                               */
+#define SMOE_W_KN 1 /* [G, K, N]: C = A W_g                                              */
+
 SMOE_API const char* smoe_version(void);
 SMOE_API const char* smoe_status_string(int status);
 /* Number of SMs of the current device (used to size persistent grids). */
@@ -143,6 +153,31 @@ SMOE_API int smoe_permute_rows(const void* x, int dtype, int T, int d, const int
 SMOE_API int smoe_combine(const void* y, int dtype, const int32_t* slot_row, const float* w, int T,
                  int k, int d, const void* shared, void* out, smoe_stream_t stream);
 
+/* ----------------------------------------------- tokens to expert rows and back
+ * The two directions of the routed rows as operators of their own, with the gate weights
+ * and what their gradients need.  slot_row, row_token and expert_offsets are those of a
+ * dispatch plan; rows_cap is the row count of `rows` / `y`; w [T,k] fp32 or NULL (all 1);
+ * k <= 32 (else SMOE_ERR_UNSUPPORTED).  Sums are fp32 in slot order, rounded once.
+ *
+ * smoe_sort_rows: rows[slot_row[t,j],:] = w[t,j] * x[t,:]; every other row of the
+ * rows_cap rows becomes zero: those from expert_offsets[E] on and, when row_token is
+ * given (plans with row_align > 1), the alignment padding.  With dw != NULL (needs w) also
+ * dw[t,j] = <x[t,:], y[slot_row[t,j],:]> (0 for slots without a row): called with x = the
+ * gradient of smoe_unsort_rows' output and y = its rows, this is that call's gradient.
+ *
+ * smoe_unsort_rows: out[t,:] = sum_j w[t,j] * y[slot_row[t,j],:] (+ residual[t,:]).  With
+ * dw != NULL (needs w) also dw[t,j] = <x[t,:], y[slot_row[t,j],:]>: the gradient of smoe_sort_rows,
+ * for y = the gradient of its rows.
+ * The reference is forward-only; these are the two directions and the gradients of its
+ * repeat_interleave / argsort dispatch and its weighted combine
+ * (models/ultimate_moe.py:118-125, 145-155; models/baseline_moe.py:166-189).          */
+SMOE_API int smoe_sort_rows(const void* x, int dtype, const int32_t* slot_row, const float* w, int T, int k, int d,
+                            const int32_t* row_token, const int32_t* expert_offsets, int E, int64_t rows_cap,
+                            void* rows, const void* y, float* dw, smoe_stream_t stream);
+SMOE_API int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const float* w, int T, int k, int d,
+                              int64_t rows_cap, const void* residual, void* out, const void* x, float* dw,
+                              smoe_stream_t stream);
+
 /* --------------------------------------------------------------------- expert GEMMs
  * Grouped GEMM over G groups of rows.  Group g owns rows [offsets[g], offsets[g+1]) of
  * A [rows_cap, K] -- or [offsets[g], ends[g]) when `ends` is not NULL -- and multiplies
@@ -177,6 +212,40 @@ SMOE_API int smoe_grouped_gemm_rows(const void* A, const void* B, const void* B3
                                     int dtype, int out_dtype, int epilogue, const int32_t* offsets,
                                     const int32_t* ends, int G, int64_t rows_cap, int N, int K,
                                     smoe_stream_t stream);
+
+/* ----------------------------------------------------------------- grouped linear layers
+ * Linear layers of G groups of rows with bias, activation and residual in the product's
+ * epilogue (one rounding to the 16-bit dtype at the end):
+ *   Z = A W_g^T + bias[g],  C = act(Z) + residual        for rows offsets[g] <= r < offsets[g+1]
+ * A [rows_cap, K], C / residual / preact [rows_cap, N], W in `w_layout` (SMOE_W_NK or, for
+ * C = A W_g, SMOE_W_KN), bias [G, N] in dtype or fp32 (bias_dtype).  bias, residual and
+ * preact may be NULL; preact receives Z rounded to dtype (the rows of the groups only).
+ * Rows of no group -- before offsets[0] or from offsets[G] on -- are left as they were, or,
+ * with fill != 0, become residual (zeros without one).  offsets are non-decreasing and live
+ * in device memory; they are clamped into [0, rows_cap].  bf16 / fp16, N and K multiples of
+ * 8, 16-byte aligned pointers, G <= 1024.  At most 2 rows stream the weights on the SIMT
+ * pipes (SMOE_W_NK), everything else runs on tcgen05 tensor cores; launches of few tiles
+ * split K over otherwise idle SMs through the workspace (its size may be 0).
+ * Replaces: nn.Linear experts with a bias around models/baseline_moe.py:151-162 (the
+ * reference's own are bias-free and linear).                                           */
+SMOE_API size_t smoe_grouped_linear_workspace_size(int64_t rows_cap, int N, int w_layout);
+SMOE_API int smoe_grouped_linear(const void* A, const void* W, int w_layout, const void* bias, int bias_dtype, int act,
+                                 const void* residual, void* preact, int fill, void* C, int dtype,
+                                 const int32_t* offsets, int G, int64_t rows_cap, int N, int K, void* workspace,
+                                 size_t workspace_bytes, smoe_stream_t stream);
+/* Element-wise part of the gradient: dz = dout * act'(preact) (rows of the groups; dz and
+ * preact unused for SMOE_ACT_NONE, where dz is dout) and, when dbias [G, N] (dtype or fp32)
+ * is not NULL, dbias[g] = the sum of the group's unrounded dz rows, in a fixed order.  The
+ * workspace is needed for dbias only.                                                  */
+SMOE_API size_t smoe_linear_act_bwd_workspace_size(int64_t rows_cap, int N, int G);
+SMOE_API int smoe_linear_act_bwd(const void* dout, const void* preact, int act, void* dz, void* dbias, int bias_dtype,
+                                 int dtype, const int32_t* offsets, int G, int64_t rows_cap, int N, void* workspace,
+                                 size_t workspace_bytes, smoe_stream_t stream);
+/* Weight gradient dW[g] = dz_g^T A_g, [G, N, K] in dtype or fp32 (out_dtype), dz
+ * [rows_cap, N], A [rows_cap, K].  Groups may start at any row; a group without rows gets
+ * zeros.  The input gradient is smoe_grouped_linear(dz, W, SMOE_W_KN).                  */
+SMOE_API int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const int32_t* offsets, int G,
+                               int64_t rows_cap, int N, int K, void* dW, int out_dtype, smoe_stream_t stream);
 
 /* out[r, :] = [lo(w[r, :]) | hi(w[r, :]) | hi(w[r, :])] for `rows` fp32 rows of K (K % 4
  * == 0, 16-byte aligned): hi = the tf32 rounding (to nearest, ties away from zero), lo =

@@ -18,6 +18,8 @@ SMOE_F32, SMOE_F16, SMOE_BF16 = 0, 1, 2
 SMOE_F32_SPLITW = 16   # layer dtype: fp32 with routed expert weights split for the tf32 tensor cores
 SMOE_EXPERT_LINEAR, SMOE_EXPERT_SWIGLU = 0, 1
 SMOE_EPI_STORE, SMOE_EPI_SWIGLU, SMOE_EPI_GATEUP = 0, 1, 3
+SMOE_W_NK, SMOE_W_KN = 0, 1
+ACT_CODE = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}   # SMOE_ACT_*
 
 DTYPE_CODE = {torch.float32: SMOE_F32, torch.float16: SMOE_F16, torch.bfloat16: SMOE_BF16}
 
@@ -69,6 +71,14 @@ SIGNATURES = {
     "smoe_dispatch_plan_noalloc": (_i32, [_vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
     "smoe_permute_rows": (_i32, [_vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _vp, _vp]),
     "smoe_combine": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "smoe_sort_rows": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _vp, _vp, _vp, _vp]),
+    "smoe_unsort_rows": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "smoe_grouped_linear_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "smoe_grouped_linear": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _i32, _i64, _i32,
+                                   _i32, _vp, _sz, _vp]),
+    "smoe_linear_act_bwd_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "smoe_linear_act_bwd": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _i64, _i32, _vp, _sz, _vp]),
+    "smoe_linear_wgrad": (_i32, [_vp, _vp, _i32, _vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp]),
     "smoe_grouped_gemm": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _vp]),
     "smoe_grouped_gemm_rows": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _vp]),
     "smoe_transpose_batched": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp]),

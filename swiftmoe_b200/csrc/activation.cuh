@@ -1,0 +1,207 @@
+// Activations of the grouped linear layers, their derivatives, and the element-wise part
+// of the layers' gradient.
+#pragma once
+#include "common.cuh"
+
+namespace smoe {
+
+// sigmoid(v) = 1 / (1 + e^-v): e^-v may be infinite, the quotient is then 0.
+__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+
+// gelu_tanh(z) = z/2 (1 + tanh u) = z sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3).
+__device__ __forceinline__ float gelu_tanh_2u(float z) {
+  constexpr float c = 1.5957691216057308f;  // 2 sqrt(2/pi)
+  return c * fmaf(0.044715f * z * z, z, z);
+}
+
+// ACT is a compile-time SMOE_ACT_*; NaN stays NaN in all of them.
+template <int ACT> __device__ __forceinline__ float act_f(float z) {
+  if constexpr (ACT == SMOE_ACT_RELU) return z < 0.0f ? 0.0f : z;
+  if constexpr (ACT == SMOE_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == SMOE_ACT_GELU_TANH) return z * sigmoid_f(gelu_tanh_2u(z));
+  if constexpr (ACT == SMOE_ACT_SILU) return z * sigmoid_f(z);
+  return z;
+}
+
+template <int ACT> __device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == SMOE_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if constexpr (ACT == SMOE_ACT_GELU)  // Phi(z) + z phi(z)
+    return fmaf(z * 0.3989422804014327f, __expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678118654752f)));
+  if constexpr (ACT == SMOE_ACT_GELU_TANH) {
+    // s + z s (1 - s) (2u)'; beyond |z| = 30 s is 0 or 1 to fp32, and the clamp keeps
+    // z^2 finite there
+    const float q = fminf(fmaxf(z, -30.0f), 30.0f);
+    const float s = sigmoid_f(gelu_tanh_2u(q));
+    const float slope = fmaf(q * s * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f * q, q, 1.0f), s);
+    return z == z ? slope : z;
+  }
+  if constexpr (ACT == SMOE_ACT_SILU) {
+    const float s = sigmoid_f(z);
+    return s * fmaf(z, 1.0f - s, 1.0f);
+  }
+  return 1.0f;
+}
+
+// f(z[i]) for a run-time activation: one uniform branch around the whole array.
+template <int N> __device__ __forceinline__ void apply_act(int act, float (&z)[N]) {
+  switch (act) {
+    case SMOE_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = act_f<SMOE_ACT_RELU>(z[i]);
+      break;
+    case SMOE_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = act_f<SMOE_ACT_GELU>(z[i]);
+      break;
+    case SMOE_ACT_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = act_f<SMOE_ACT_GELU_TANH>(z[i]);
+      break;
+    case SMOE_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = act_f<SMOE_ACT_SILU>(z[i]);
+      break;
+    default: break;
+  }
+}
+
+// What the epilogue of a grouped linear layer adds to its products: out = act(acc +
+// bias[g]) + residual[row], preact[row] = acc + bias[g] (kept for the gradient).  Null
+// pointers leave a term out.  Column counts are multiples of 8, pointers 16-byte aligned.
+struct LinearEpi {
+  const void* bias = nullptr;      // [G, N], the layer's 16-bit type, or fp32
+  const void* residual = nullptr;  // [rows_cap, N], the layer's type
+  void* preact = nullptr;          // [rows_cap, N], the layer's type
+  int bias_f32 = 0;
+  int act = SMOE_ACT_NONE;
+  int fill = 0;                    // rows of no group get residual (or 0) instead of staying as they were
+};
+
+// v[i] += bias[g, col + i] for W consecutive columns (W = 4 or a multiple of 8).
+template <typename T, int W>
+__device__ __forceinline__ void add_bias(const LinearEpi& lin, int64_t at, float (&v)[W]) {
+  if (lin.bias == nullptr) return;
+  if (lin.bias_f32) {
+    const float* b = static_cast<const float*>(lin.bias) + at;
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(b) + i);
+      v[4 * i] += q.x;
+      v[4 * i + 1] += q.y;
+      v[4 * i + 2] += q.z;
+      v[4 * i + 3] += q.w;
+    }
+  } else {
+    const T* b = static_cast<const T*>(lin.bias) + at;
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+      const uint2 q = __ldg(reinterpret_cast<const uint2*>(b) + i);
+      const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * i + j] += Num<T>::to_f(e[j]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ gradient, element-wise
+// dz = dout * act'(z) for the rows of the groups, and the bias gradient db[g] = the sum
+// of dz over the group's rows, from the unrounded fp32 products.  Memory-bound: dout and
+// z read once, dz written once.  A block owns 256 columns (a lane 8 of them) of `slice`
+// consecutive rows, its eight warps every eighth row; it walks the groups its rows belong
+// to and writes one partial row of column sums per group to part[s + g], which is a
+// different row for every (slice s, group g) pair that has rows, since both only grow
+// along the rows.  bias_grad_reduce_kernel adds a group's partials in slice order, so no
+// result depends on the order in which blocks run.
+constexpr int kActCols = 256;
+
+template <typename T, int ACT, bool BIAS>
+__global__ void __launch_bounds__(256) linear_act_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ z,
+                                                             T* __restrict__ dz, const int32_t* __restrict__ offsets,
+                                                             int G, int rows_cap, int N, int slice,
+                                                             float* __restrict__ part) {
+  __shared__ float s_sum[8][kActCols + 8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = blockIdx.x * kActCols + lane * 8;
+  const bool live = col < N;
+  const int end_all = min(max(offsets[G], 0), rows_cap);
+  int row = max(blockIdx.y * slice, max(offsets[0], 0));
+  const int row_end = min((int)blockIdx.y * slice + slice, end_all);
+  if (row >= row_end) return;
+  int lo = 0, hi = G - 1;  // last group whose start <= row
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (offsets[mid] <= row) lo = mid; else hi = mid - 1;
+  }
+  for (int g = lo; g < G && row < row_end; ++g) {
+    const int stop = min(offsets[g + 1], row_end);
+    if (stop <= row) continue;
+    float sum[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+    if (live) {
+#pragma unroll 4
+      for (int r = row + warp; r < stop; r += 8) {
+        float dy[8];
+        load_vec_f<T, 8>(dout + (int64_t)r * N + col, dy);
+        if constexpr (ACT != SMOE_ACT_NONE) {
+          float zz[8];
+          load_vec_f<T, 8>(z + (int64_t)r * N + col, zz);
+          union {
+            uint4 u;
+            T e[8];
+          } o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            dy[i] *= act_slope<ACT>(zz[i]);
+            o.e[i] = Num<T>::from_f(dy[i]);
+          }
+          *reinterpret_cast<uint4*>(dz + (int64_t)r * N + col) = o.u;
+        }
+        if constexpr (BIAS)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[i] += dy[i];
+      }
+    }
+    if constexpr (BIAS) {
+      __syncthreads();  // the previous group's sums have been read
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s_sum[warp][lane * 8 + i] = sum[i];
+      __syncthreads();
+      const int c = blockIdx.x * kActCols + threadIdx.x;
+      if (c < N) {
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s += s_sum[q][threadIdx.x];
+        part[((int64_t)blockIdx.y + g) * N + c] = s;
+      }
+    }
+    row = stop;
+  }
+}
+
+// dbias[g, n] = sum over the group's slices, in order; OutT is the bias's type.  One block:
+// 32 columns of one group, each of its eight warps every eighth slice, then the eight sums
+// in warp order.
+template <typename OutT>
+__global__ void __launch_bounds__(256) bias_grad_reduce_kernel(const float* __restrict__ part,
+                                                               const int32_t* __restrict__ offsets, int G, int rows_cap,
+                                                               int N, int slice, OutT* __restrict__ dbias) {
+  __shared__ float s_sum[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane, g = blockIdx.y;
+  const int b = min(max(offsets[g], 0), rows_cap), e = min(max(offsets[g + 1], b), rows_cap);
+  float s = 0.f;
+  if (c < N && e > b)
+#pragma unroll 4
+    for (int q = b / slice + warp; q <= (e - 1) / slice; q += 8) s += part[((int64_t)q + g) * N + c];
+  s_sum[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < N) {
+    float t = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) t += s_sum[q][lane];
+    dbias[(int64_t)g * N + c] = Num<OutT>::from_f(t);
+  }
+}
+
+}  // namespace smoe

@@ -8,8 +8,10 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <mutex>
+#include <type_traits>
 #include <utility>
 
 #include "common.cuh"
@@ -19,6 +21,7 @@
 #include "gemm_simt.cuh"
 #include "gemv.cuh"
 #include "gemm_tc.cuh"
+#include "routed_rows.cuh"
 #include "router.cuh"
 
 using namespace smoe;
@@ -314,18 +317,19 @@ void* tf32_scratch(cudaStream_t st, size_t bytes) {
 
 // forced: a split-K scratch of the caller's with at least min_split slices per tile;
 // otherwise the stream's own (the kernel then splits only launches with few tiles).
-template <int EPI, typename OutT, int ES = 2>
+template <int EPI, typename OutT, int ES = 2, bool BMN = false>
 int launch_tc(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb3, void* C, int64_t ldc,
               const uint64_t* row_ptrs, const int32_t* offsets, const int32_t* ends, int G, int64_t rows_cap, int N, int K, uint32_t idesc,
-              cudaStream_t st, const SplitScratch* forced = nullptr, int min_split = 1) {
+              cudaStream_t st, const SplitScratch* forced = nullptr, int min_split = 1,
+              const LinearEpi& lin = LinearEpi()) {
   static SmemGrant done;
-  auto kern = tc::grouped_gemm_kernel<EPI, OutT, ES>;
+  auto kern = tc::grouped_gemm_kernel<EPI, OutT, ES, BMN>;
   constexpr int smem = EPI == tc::EPI_ROWS ? tc::SMEM_BYTES_ROWS : tc::SMEM_BYTES;
   SMOE_CK(ensure_smem(kern, smem, &done));
   const SplitScratch sc = forced ? *forced : split_scratch(st);
   SMOE_CK(launch_k(kern, device_sms(), tc::THREADS, smem, st, ma, mb, mb3, reinterpret_cast<OutT*>(C), ldc, row_ptrs, offsets, ends, G, N,
                                                          K, (int)rows_cap, raster_band(EPI), idesc, sc.ws, sc.cnt, sc.units,
-                                                         forced ? min_split : 1));
+                                                         forced ? min_split : 1, lin));
   SMOE_CK(cudaGetLastError());
   return SMOE_OK;
 }
@@ -344,16 +348,16 @@ int launch_tc_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorM
   return SMOE_OK;
 }
 
-template <bool MN>
-int launch_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, float* C, const int32_t* koff, int G, int M, int N,
-                 uint32_t idesc, cudaStream_t st) {
+template <bool MN, typename OutT = float, bool ANY = false>
+int launch_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, OutT* C, const int32_t* koff, int G, int M, int N,
+                 uint32_t idesc, cudaStream_t st, int k_rows = 0) {
   static SmemGrant done;
-  auto kern = tc::wgrad_gemm_kernel<float, MN>;
+  auto kern = tc::wgrad_gemm_kernel<OutT, MN, ANY>;
   SMOE_CK(ensure_smem(kern, tc::SMEM_BYTES_ROWS, &done));
   const int64_t tiles = (int64_t)G * cdiv(M, tc::BM) * cdiv(N, tc::BN);
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sms()));
   // keep the smaller operand (per group: N rows of B against M rows of A) in L2
-  kern<<<grid, tc::THREADS, tc::SMEM_BYTES_ROWS, st>>>(ma, mb, C, koff, G, M, N, idesc, N <= M);
+  kern<<<grid, tc::THREADS, tc::SMEM_BYTES_ROWS, st>>>(ma, mb, C, koff, G, M, N, idesc, N <= M, k_rows);
   SMOE_CK(cudaGetLastError());
   return SMOE_OK;
 }
@@ -361,7 +365,7 @@ int launch_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, float* C, const i
 template <int EPI, typename T, typename OutT>
 int launch_gemv_t(const void* A, const void* B, const void* B3, void* C, const uint64_t* row_ptrs,
                   const int32_t* offsets, const int32_t* ends, int G, int64_t rows_cap, int N, int K,
-                  cudaStream_t st, const int32_t* a_index, int a_rows) {
+                  cudaStream_t st, const int32_t* a_index, int a_rows, const LinearEpi& lin = LinearEpi()) {
   // one warp (two for rows of 8192 or more elements) per (group with rows, column); at
   // most min(G, rows_cap) groups have rows.  Measured on the Mixtral decode shapes: two
   // warps take the 14336-element down rows in 54 us (one: 60, four: 57); the 4096-element
@@ -372,13 +376,13 @@ int launch_gemv_t(const void* A, const void* B, const void* B3, void* C, const u
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv(cols, CPB), 65535));
     SMOE_CK(launch_k(gemv::grouped_gemv_kernel<EPI, T, OutT, 2>, grid, gemv::THREADS, 0, st, 
         (const T*)A, (const T*)B, (const T*)B3, (OutT*)C, N, row_ptrs, offsets, ends, G, N, K, (int)rows_cap, a_index,
-        a_rows));
+        a_rows, lin));
   } else {
     const unsigned grid = (unsigned)std::max<int64_t>(
         1, std::min<int64_t>(cdiv(cols * 32, gemv::THREADS), (int64_t)device_sms() * 8));
     SMOE_CK(launch_k(gemv::grouped_gemv_kernel<EPI, T, OutT, 1>, grid, gemv::THREADS, 0, st, 
         (const T*)A, (const T*)B, (const T*)B3, (OutT*)C, N, row_ptrs, offsets, ends, G, N, K, (int)rows_cap, a_index,
-        a_rows));
+        a_rows, lin));
   }
   SMOE_CK(cudaGetLastError());
   return SMOE_OK;
@@ -586,6 +590,124 @@ int grouped_gemm_impl(const void* A, const void* B, const void* B3, void* C, int
   if (out_dtype == SMOE_F32) return launch_tc<SMOE_EPI_STORE, float>(ma, mb, mb3, C, N, row_ptrs, offsets, ends, G, rows_cap, N, K, idesc, st);
   return dtype == SMOE_BF16 ? launch_tc<SMOE_EPI_STORE, __nv_bfloat16>(ma, mb, mb3, C, N, row_ptrs, offsets, ends, G, rows_cap, N, K, idesc, st)
                             : launch_tc<SMOE_EPI_STORE, __half>(ma, mb, mb3, C, N, row_ptrs, offsets, ends, G, rows_cap, N, K, idesc, st);
+}
+
+// ------------------------------------------------------------------ grouped linear layers
+// 3-D map over [G, K, N] weights read along N: box = 64 columns (N) x 64 rows (K) x 1 group,
+// an MN-major operand tile.
+bool make_map_3d_mn(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int64_t G, int64_t K, int64_t N) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)N, (cuuint64_t)K, (cuuint64_t)G};
+  cuuint64_t strides[2] = {(cuuint64_t)N * 2, (cuuint64_t)N * K * 2};
+  cuuint32_t box[3] = {64, tc::BK, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Split-K scratch of a linear layer: the caller's workspace, so that graphs captured on
+// one stream and replayed on several never share it.  Wanted where the rows, were they all
+// of one group, would make at most half as many tiles as SMs (the kernel's own condition,
+// on the device, is the same on the groups' real tiles).
+constexpr size_t kSplitSlot = (size_t)tc::BM * tc::BN * sizeof(float);
+size_t linear_workspace(int64_t rows_cap, int N) {
+  const int units = device_sms();
+  if (rows_cap < 1 || 2 * cdiv(rows_cap, tc::BM) * cdiv(N, tc::BN) > units) return 0;
+  return (size_t)units * (kSplitSlot + sizeof(int));
+}
+
+template <typename T, bool BMN>
+int linear_gemm_t(const void* A, const void* B, void* C, const int32_t* offsets, int G, int64_t rows_cap, int N, int K,
+                  const LinearEpi& lin, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+  if (!BMN && rows_cap <= gemv::DISPATCH_ROWS)  // decode: the weights of the groups with rows, streamed once
+    return launch_gemv_t<gemv::EPI_LINEAR, T, T>(A, B, nullptr, C, nullptr, offsets, nullptr, G, rows_cap, N, K, st,
+                                                 nullptr, (int)rows_cap, lin);
+  const CUtensorMapDataType dt = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap ma, mb;
+  if (!make_map_2d(&ma, A, dt, rows_cap, K)) return SMOE_ERR_CUDA;
+  if (BMN ? !make_map_3d_mn(&mb, B, dt, G, K, N) : !make_map_3d(&mb, B, dt, G, N, K)) return SMOE_ERR_CUDA;
+  const uint32_t idesc = umma_idesc_f16(bf ? 1u : 0u, tc::BM, tc::BN) | (BMN ? 1u << 16 : 0u);  // transpose-B bit
+  SplitScratch sc;  // without units: no split
+  const size_t need = linear_workspace(rows_cap, N);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need) return SMOE_ERR_WORKSPACE;
+    sc.units = device_sms();
+    sc.ws = static_cast<float*>(workspace);
+    sc.cnt = reinterpret_cast<int*>(static_cast<char*>(workspace) + (size_t)sc.units * kSplitSlot);
+    SMOE_CK(cudaMemsetAsync(sc.cnt, 0, (size_t)sc.units * sizeof(int), st));
+  }
+  return launch_tc<tc::EPI_LINEAR, T, 2, BMN>(ma, mb, mb, C, N, nullptr, offsets, nullptr, G, rows_cap, N, K, idesc, st,
+                                              &sc, 1, lin);
+}
+
+// Rows of a bias-gradient partial sum: enough slices to fill the GPU, at most 64 of them.
+int act_bwd_slice(int64_t rows_cap) { return (int)std::max<int64_t>(64, align_up((size_t)cdiv(rows_cap, 64), 64)); }
+
+template <typename T, bool BIAS>
+cudaError_t launch_act_bwd(const void* dout, const void* z, void* dz, int act, const int32_t* offsets, int G,
+                           int64_t rows_cap, int N, int slice, float* part, cudaStream_t st) {
+  const dim3 grid((unsigned)cdiv(N, kActCols), (unsigned)cdiv(rows_cap, slice));
+#define SMOE_ACT_BWD(ACT)                                                                                        \
+  return launch_k(linear_act_bwd_kernel<T, ACT, BIAS>, grid, 256, 0, st, (const T*)dout, (const T*)z, (T*)dz, offsets, \
+                  G, (int)rows_cap, N, slice, part)
+  switch (act) {
+    case SMOE_ACT_RELU: SMOE_ACT_BWD(SMOE_ACT_RELU);
+    case SMOE_ACT_GELU: SMOE_ACT_BWD(SMOE_ACT_GELU);
+    case SMOE_ACT_GELU_TANH: SMOE_ACT_BWD(SMOE_ACT_GELU_TANH);
+    case SMOE_ACT_SILU: SMOE_ACT_BWD(SMOE_ACT_SILU);
+    default:
+      if constexpr (BIAS) SMOE_ACT_BWD(SMOE_ACT_NONE);
+      return cudaSuccess;  // dz is dout
+  }
+#undef SMOE_ACT_BWD
+}
+
+// ------------------------------------------------------------------ tokens <-> rows
+// One warp per token, or, for batches of fewer tokens than would fill the GPU that way,
+// the eight warps of a block.
+int token_warps(int T) { return T <= 4 * device_sms() ? 8 : 1; }
+unsigned token_grid(int T, int wpt) {
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv((int64_t)T * wpt, rows::WARPS), (int64_t)device_sms() * 8));
+}
+
+template <typename T, int VEC, int WPT>
+cudaError_t launch_sort_rows(const void* x, const int32_t* sr, const float* w, int T_, int k, int d,
+                             const int32_t* row_token, const int32_t* offsets, int E, int64_t rows_cap, void* out,
+                             const void* y, float* dw, cudaStream_t st) {
+  const unsigned grid = token_grid(T_, WPT);
+#define SMOE_SORT(HW, DOT)                                                                                          \
+  return launch_k(rows::sort_rows_kernel<T, VEC, WPT, HW, DOT>, grid, rows::THREADS, 0, st, (const T*)x, sr, w, T_, k, \
+                  d, row_token, offsets, E, rows_cap, (T*)out, (const T*)y, dw)
+  if (dw) SMOE_SORT(true, true);
+  if (w) SMOE_SORT(true, false);
+  SMOE_SORT(false, false);
+#undef SMOE_SORT
+}
+
+template <typename T, int VEC, int WPT>
+cudaError_t launch_unsort_rows(const void* y, const int32_t* sr, const float* w, int T_, int k, int d,
+                               int64_t rows_cap, const void* residual, void* out, const void* x, float* dw,
+                               cudaStream_t st) {
+  const unsigned grid = token_grid(T_, WPT);
+#define SMOE_UNSORT(HW, DOT)                                                                                      \
+  return launch_k(rows::unsort_rows_kernel<T, VEC, WPT, HW, DOT>, grid, rows::THREADS, 0, st, (const T*)y, sr, w, T_, \
+                  k, d, rows_cap, (const T*)residual, (T*)out, (const T*)x, dw)
+  if (dw) SMOE_UNSORT(true, true);
+  if (w) SMOE_UNSORT(true, false);
+  SMOE_UNSORT(false, false);
+#undef SMOE_UNSORT
+}
+
+// Elements per load: 16 bytes where rows start on 16-byte boundaries, 4 bytes (two 16-bit
+// elements) where they start on 4-byte ones, else single elements.
+int row_vec(int es, int d, std::initializer_list<const void*> ptrs) {
+  uintptr_t a = (uintptr_t)d * es;
+  for (const void* p : ptrs) a |= reinterpret_cast<uintptr_t>(p);
+  if ((a & 15) == 0) return 16 / es;
+  return (a & 3) == 0 && es == 2 ? 2 : 1;
 }
 
 // ------------------------------------------------------------------ router
@@ -929,6 +1051,171 @@ int smoe_combine(const void* y, int dtype, const int32_t* slot_row, const float*
 #undef SMOE_COMBINE
   SMOE_CK(cudaGetLastError());
   return SMOE_OK;
+}
+
+#define SMOE_ROWS_CASE(TY, VV)                              \
+  SMOE_CK(wpt == 1 ? SMOE_ROWS_LAUNCH(TY, VV, 1) : SMOE_ROWS_LAUNCH(TY, VV, 8))
+#define SMOE_ROWS_DISPATCH()                                \
+  switch (dtype) {                                          \
+    case SMOE_F32:                                          \
+      if (vec == 4) SMOE_ROWS_CASE(float, 4);               \
+      else SMOE_ROWS_CASE(float, 1);                        \
+      break;                                                \
+    case SMOE_F16:                                          \
+      if (vec == 8) SMOE_ROWS_CASE(__half, 8);              \
+      else if (vec == 2) SMOE_ROWS_CASE(__half, 2);         \
+      else SMOE_ROWS_CASE(__half, 1);                       \
+      break;                                                \
+    default:                                                \
+      if (vec == 8) SMOE_ROWS_CASE(__nv_bfloat16, 8);       \
+      else if (vec == 2) SMOE_ROWS_CASE(__nv_bfloat16, 2);  \
+      else SMOE_ROWS_CASE(__nv_bfloat16, 1);                \
+  }
+
+int smoe_sort_rows(const void* x, int dtype, const int32_t* slot_row, const float* w, int T, int k, int d,
+                   const int32_t* row_token, const int32_t* expert_offsets, int E, int64_t rows_cap, void* rows,
+                   const void* y, float* dw, smoe_stream_t stream) {
+  const int es = elt_size(dtype);
+  if (es == 0 || T < 0 || k < 1 || d < 1 || E < 1 || rows_cap < 0) return SMOE_ERR_INVALID;
+  if (k > rows::MAX_K || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (T == 0 && rows_cap == 0) return SMOE_OK;
+  if (!expert_offsets || (rows_cap > 0 && !rows) || (T > 0 && (!x || !slot_row)) || (dw && (!w || (rows_cap > 0 && !y))))
+    return SMOE_ERR_INVALID;
+  const int vec = row_vec(es, d, {x, rows, dw ? y : nullptr}), wpt = token_warps(T);
+  cudaStream_t st = (cudaStream_t)stream;
+#define SMOE_ROWS_LAUNCH(TY, VV, WW) \
+  (launch_sort_rows<TY, VV, WW>(x, slot_row, w, T, k, d, row_token, expert_offsets, E, rows_cap, rows, y, dw, st))
+  SMOE_ROWS_DISPATCH();
+#undef SMOE_ROWS_LAUNCH
+  SMOE_CK(cudaGetLastError());
+  return SMOE_OK;
+}
+
+int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const float* w, int T, int k, int d,
+                     int64_t rows_cap, const void* residual, void* out, const void* x, float* dw,
+                     smoe_stream_t stream) {
+  const int es = elt_size(dtype);
+  if (es == 0 || T < 0 || k < 1 || d < 1 || rows_cap < 0) return SMOE_ERR_INVALID;
+  if (k > rows::MAX_K || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (T == 0) return SMOE_OK;
+  if (!slot_row || !out || (rows_cap > 0 && !y) || (dw && (!w || !x))) return SMOE_ERR_INVALID;
+  const int vec = row_vec(es, d, {y, out, residual, dw ? x : nullptr}), wpt = token_warps(T);
+  cudaStream_t st = (cudaStream_t)stream;
+#define SMOE_ROWS_LAUNCH(TY, VV, WW) \
+  (launch_unsort_rows<TY, VV, WW>(y, slot_row, w, T, k, d, rows_cap, residual, out, x, dw, st))
+  SMOE_ROWS_DISPATCH();
+#undef SMOE_ROWS_LAUNCH
+  SMOE_CK(cudaGetLastError());
+  return SMOE_OK;
+}
+#undef SMOE_ROWS_DISPATCH
+#undef SMOE_ROWS_CASE
+
+size_t smoe_grouped_linear_workspace_size(int64_t rows_cap, int N, int w_layout) {
+  if (rows_cap < 1 || N < 1 || (w_layout == SMOE_W_NK && rows_cap <= gemv::DISPATCH_ROWS)) return 0;
+  return linear_workspace(rows_cap, N);
+}
+
+int smoe_grouped_linear(const void* A, const void* W, int w_layout, const void* bias, int bias_dtype, int act,
+                        const void* residual, void* preact, int fill, void* C, int dtype, const int32_t* offsets, int G,
+                        int64_t rows_cap, int N, int K, void* workspace, size_t workspace_bytes,
+                        smoe_stream_t stream) {
+  if (G < 1 || N < 1 || K < 1 || rows_cap < 0 || act < SMOE_ACT_NONE || act > SMOE_ACT_SILU) return SMOE_ERR_INVALID;
+  if (w_layout != SMOE_W_NK && w_layout != SMOE_W_KN) return SMOE_ERR_INVALID;
+  if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_UNSUPPORTED;
+  if (bias && bias_dtype != dtype && bias_dtype != SMOE_F32) return SMOE_ERR_UNSUPPORTED;
+  if (N % 8 != 0 || K % 8 != 0 || G > tc::MAX_GROUPS || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (rows_cap == 0) return SMOE_OK;
+  if (!A || !W || !C || !offsets) return SMOE_ERR_INVALID;
+  for (const void* p : {A, W, bias, residual, (const void*)preact, (const void*)C, (const void*)workspace})
+    if (!aligned16(p)) return SMOE_ERR_UNSUPPORTED;
+  LinearEpi lin;
+  lin.bias = bias;
+  lin.bias_f32 = bias && bias_dtype == SMOE_F32;
+  lin.act = act;
+  lin.residual = residual;
+  lin.preact = preact;
+  lin.fill = fill != 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (w_layout == SMOE_W_KN)
+    return dtype == SMOE_BF16 ? linear_gemm_t<__nv_bfloat16, true>(A, W, C, offsets, G, rows_cap, N, K, lin, workspace,
+                                                       workspace_bytes, st)
+                              : linear_gemm_t<__half, true>(A, W, C, offsets, G, rows_cap, N, K, lin, workspace,
+                                                       workspace_bytes, st);
+  return dtype == SMOE_BF16 ? linear_gemm_t<__nv_bfloat16, false>(A, W, C, offsets, G, rows_cap, N, K, lin, workspace,
+                                                       workspace_bytes, st)
+                            : linear_gemm_t<__half, false>(A, W, C, offsets, G, rows_cap, N, K, lin, workspace,
+                                                       workspace_bytes, st);
+}
+
+size_t smoe_linear_act_bwd_workspace_size(int64_t rows_cap, int N, int G) {
+  if (rows_cap < 1 || N < 1 || G < 1) return 0;
+  return (size_t)(cdiv(rows_cap, act_bwd_slice(rows_cap)) + G) * N * sizeof(float);
+}
+
+int smoe_linear_act_bwd(const void* dout, const void* preact, int act, void* dz, void* dbias, int bias_dtype, int dtype,
+                        const int32_t* offsets, int G, int64_t rows_cap, int N, void* workspace, size_t workspace_bytes,
+                        smoe_stream_t stream) {
+  if (G < 1 || N < 1 || rows_cap < 0 || act < SMOE_ACT_NONE || act > SMOE_ACT_SILU) return SMOE_ERR_INVALID;
+  if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_UNSUPPORTED;
+  if (dbias && bias_dtype != dtype && bias_dtype != SMOE_F32) return SMOE_ERR_UNSUPPORTED;
+  if (N % 8 != 0 || G > tc::MAX_GROUPS || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (rows_cap == 0) {
+    if (dbias) SMOE_CK(cudaMemsetAsync(dbias, 0, (size_t)G * N * elt_size(bias_dtype), st));
+    return SMOE_OK;
+  }
+  if (act == SMOE_ACT_NONE && !dbias) return SMOE_OK;
+  if (!dout || !offsets || (act != SMOE_ACT_NONE && (!preact || !dz))) return SMOE_ERR_INVALID;
+  for (const void* p : {dout, preact, (const void*)dz, (const void*)dbias})
+    if (!aligned16(p)) return SMOE_ERR_UNSUPPORTED;
+  if (dbias && (!workspace || workspace_bytes < smoe_linear_act_bwd_workspace_size(rows_cap, N, G)))
+    return SMOE_ERR_WORKSPACE;
+  const int slice = act_bwd_slice(rows_cap);
+  float* part = static_cast<float*>(workspace);
+  const bool bf = dtype == SMOE_BF16;
+  if (!dbias) {
+    SMOE_CK(bf ? (launch_act_bwd<__nv_bfloat16, false>(dout, preact, dz, act, offsets, G, rows_cap, N, slice, part, st))
+               : (launch_act_bwd<__half, false>(dout, preact, dz, act, offsets, G, rows_cap, N, slice, part, st)));
+    return SMOE_OK;
+  }
+  SMOE_CK(bf ? (launch_act_bwd<__nv_bfloat16, true>(dout, preact, dz, act, offsets, G, rows_cap, N, slice, part, st))
+             : (launch_act_bwd<__half, true>(dout, preact, dz, act, offsets, G, rows_cap, N, slice, part, st)));
+  const dim3 grid((unsigned)cdiv(N, 32), (unsigned)G);
+  if (bias_dtype == SMOE_F32)
+    SMOE_CK(launch_k(bias_grad_reduce_kernel<float>, grid, 256, 0, st, part, offsets, G, (int)rows_cap, N, slice, (float*)dbias));
+  else if (bf)
+    SMOE_CK(launch_k(bias_grad_reduce_kernel<__nv_bfloat16>, grid, 256, 0, st, part, offsets, G, (int)rows_cap, N, slice,
+                     (__nv_bfloat16*)dbias));
+  else
+    SMOE_CK(launch_k(bias_grad_reduce_kernel<__half>, grid, 256, 0, st, part, offsets, G, (int)rows_cap, N, slice, (__half*)dbias));
+  return SMOE_OK;
+}
+
+int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const int32_t* offsets, int G, int64_t rows_cap, int N,
+                      int K, void* dW, int out_dtype, smoe_stream_t stream) {
+  if (G < 1 || N < 1 || K < 1 || rows_cap < 0 || !offsets || !dW) return SMOE_ERR_INVALID;
+  if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_UNSUPPORTED;
+  if (out_dtype != dtype && out_dtype != SMOE_F32) return SMOE_ERR_UNSUPPORTED;
+  if (N % 8 != 0 || K % 8 != 0 || G > tc::MAX_GROUPS || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (rows_cap == 0) {
+    SMOE_CK(cudaMemsetAsync(dW, 0, (size_t)G * N * K * elt_size(out_dtype), st));
+    return SMOE_OK;
+  }
+  if (!dz || !A) return SMOE_ERR_INVALID;
+  if (!aligned16(dz) || !aligned16(A) || !aligned16(dW)) return SMOE_ERR_UNSUPPORTED;
+  if ((int64_t)G * cdiv(N, tc::BM) * cdiv(K, tc::BN) > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  const bool bf = dtype == SMOE_BF16;
+  const CUtensorMapDataType dt = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap ma, mb;
+  if (!make_map_2d_box(&ma, dz, dt, rows_cap, N, N, tc::BK)) return SMOE_ERR_CUDA;
+  if (!make_map_2d_box(&mb, A, dt, rows_cap, K, K, tc::BK)) return SMOE_ERR_CUDA;
+  const uint32_t idesc = umma_idesc_f16_mn(bf ? 1u : 0u, tc::BM, tc::BN);
+  const int kr = (int)rows_cap;
+  if (out_dtype == SMOE_F32) return launch_wgrad<true, float, true>(ma, mb, (float*)dW, offsets, G, N, K, idesc, st, kr);
+  return bf ? launch_wgrad<true, __nv_bfloat16, true>(ma, mb, (__nv_bfloat16*)dW, offsets, G, N, K, idesc, st, kr)
+            : launch_wgrad<true, __half, true>(ma, mb, (__half*)dW, offsets, G, N, K, idesc, st, kr);
 }
 
 int smoe_grouped_gemm(const void* A, const void* B, const void* B3, void* C, int dtype, int out_dtype, int epilogue,

@@ -4,6 +4,7 @@ entry point on the current CUDA stream.  They never fall back to another
 implementation: a non-CUDA tensor or a failed call raises."""
 from __future__ import annotations
 
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -22,6 +23,18 @@ def _need_cuda(*ts):
 
 def _workspace(device, nbytes: int) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+
+
+def _same_device(device, *ts):
+    for t in ts:
+        if t is not None and t.device != device:
+            raise L.SwiftMoEError(f"tensors on different devices: {device} and {t.device}")
+
+
+def _on(device):
+    """The device the launch belongs to, made current if it is not (streams and tensors of
+    another GPU than the current one)."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def router(x: torch.Tensor, gate_w: torch.Tensor, k: int, logit_bias: Optional[torch.Tensor] = None,
@@ -57,7 +70,8 @@ def topk_from_logits(logits: torch.Tensor, k: int):
 
 
 def dispatch_plan(idx: torch.Tensor, num_experts: int, capacity: int = 0, row_align: int = 1):
-    """Returns dict(counts [E], offsets [E+1], slot_row [T*k], row_token [rows_cap], rows_cap)."""
+    """Returns dict(counts [E], offsets [E+1], slot_row [T*k], row_token [rows_cap], rows_cap,
+    T, k, row_align)."""
     _need_cuda(idx)
     if idx.dtype != torch.int32:
         raise L.SwiftMoEError("idx must be int32")
@@ -74,7 +88,8 @@ def dispatch_plan(idx: torch.Tensor, num_experts: int, capacity: int = 0, row_al
     L.check(lib.smoe_dispatch_plan(L.ptr(idx), T, k, E, capacity, row_align, L.ptr(counts), L.ptr(offsets),
                                    L.ptr(slot_row), L.ptr(row_token), max(rows_cap, 1), L.ptr(ws), ws.numel(),
                                    L.stream_handle(dev)), "smoe_dispatch_plan")
-    return dict(counts=counts, offsets=offsets, slot_row=slot_row, row_token=row_token, rows_cap=rows_cap)
+    return dict(counts=counts, offsets=offsets, slot_row=slot_row, row_token=row_token, rows_cap=rows_cap, T=T, k=k,
+                row_align=row_align)
 
 
 def permute_rows(x: torch.Tensor, row_token: torch.Tensor, offsets: torch.Tensor, rows_cap: int,
@@ -108,6 +123,178 @@ def combine(y: torch.Tensor, slot_row: torch.Tensor, w: torch.Tensor, T: int, k:
     L.check(L.load().smoe_combine(L.ptr(y), L.dtype_code(y.dtype), L.ptr(slot_row), L.ptr(w), T, k, d,
                                   L.ptr(shared), L.ptr(out), L.stream_handle(y.device)), "smoe_combine")
     return out
+
+
+def _plan_args(plan: dict, rows: int, device, w: Optional[torch.Tensor]):
+    """(slot_row, T, k) of a dispatch plan after checking that it fits `rows` rows and w."""
+    slot_row, T, k = plan["slot_row"], plan["T"], plan["k"]
+    _need_cuda(slot_row, plan["offsets"], w)
+    _same_device(device, slot_row, plan["offsets"], w)
+    if slot_row.dtype != torch.int32 or plan["offsets"].dtype != torch.int32 or slot_row.numel() != T * k:
+        raise L.SwiftMoEError("not a dispatch plan: slot_row must be int32 [T*k], offsets int32")
+    if rows < plan["rows_cap"]:
+        raise L.SwiftMoEError(f"the plan has up to {plan['rows_cap']} rows, the tensor only {rows}")
+    if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (T, k)):
+        raise L.SwiftMoEError(f"weights must be float32 [{T}, {k}], got {w.dtype} {tuple(w.shape)}")
+    return slot_row, T, k
+
+
+def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, rows_cap: Optional[int] = None,
+              y: Optional[torch.Tensor] = None):
+    """rows [rows_cap, d] with rows[slot_row[t,j]] = (w[t,j] *) x[t]; all other rows (padding,
+    rows behind the last expert's) are zero.  rows_cap: the plan's unless given.
+
+    With ``y`` [rows_cap, d] (needs w) returns (rows, dw [T,k] fp32), dw[t,j] = <x[t],
+    y[slot_row[t,j]]>: for x = the gradient of ``unsort_rows``' output and y = its rows
+    these are its gradients."""
+    _need_cuda(x, y)
+    rows_cap = plan["rows_cap"] if rows_cap is None else rows_cap
+    slot_row, T, k = _plan_args(plan, rows_cap, x.device, w)
+    row_token = plan["row_token"] if plan.get("row_align") != 1 else None
+    _need_cuda(row_token)
+    _same_device(x.device, y, row_token)
+    if x.dim() != 2 or x.shape[0] != T:
+        raise L.SwiftMoEError(f"the plan is for {T} tokens, got x of shape {tuple(x.shape)}")
+    if row_token is not None and (row_token.dtype != torch.int32 or row_token.numel() < plan["rows_cap"]):
+        raise L.SwiftMoEError("not a dispatch plan: row_token must be int32 [rows_cap]")
+    d = x.shape[1]
+    if y is not None and (w is None or y.dtype != x.dtype or tuple(y.shape) != (rows_cap, d)):
+        raise L.SwiftMoEError("y needs weights, x's dtype and shape [rows_cap, d]")
+    rows = torch.empty((rows_cap, d), dtype=x.dtype, device=x.device)
+    dw = torch.empty((T, k), dtype=torch.float32, device=x.device) if y is not None else None
+    with _on(x.device):
+        L.check(L.load().smoe_sort_rows(L.ptr(x), L.dtype_code(x.dtype), L.ptr(slot_row), L.ptr(w), T, k, d,
+                                        L.ptr(row_token), L.ptr(plan["offsets"]), plan["offsets"].numel() - 1, rows_cap,
+                                        L.ptr(rows), L.ptr(y), L.ptr(dw), L.stream_handle(x.device)), "smoe_sort_rows")
+    return rows if y is None else (rows, dw)
+
+
+def unsort_rows(y: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                *, x: Optional[torch.Tensor] = None):
+    """out [T, d] with out[t] = sum_j (w[t,j] *) y[slot_row[t,j]] (+ residual[t]), summed in
+    slot order in fp32, rounded once.
+
+    With ``x`` [T, d] (needs w) returns (out, dw [T,k] fp32), dw[t,j] = <x[t],
+    y[slot_row[t,j]]>: for y = the gradient of ``sort_rows``' rows and x = its input these
+    are its gradients."""
+    _need_cuda(y, residual, x)
+    _same_device(y.device, residual, x)
+    if y.dim() != 2:
+        raise L.SwiftMoEError(f"rows must be [rows, d], got {tuple(y.shape)}")
+    rows_cap, d = y.shape
+    slot_row, T, k = _plan_args(plan, rows_cap, y.device, w)
+    for name, t in (("residual", residual), ("x", x)):
+        if t is not None and (t.dtype != y.dtype or tuple(t.shape) != (T, d)):
+            raise L.SwiftMoEError(f"{name} must be {y.dtype} [{T}, {d}], got {t.dtype} {tuple(t.shape)}")
+    if x is not None and w is None:
+        raise L.SwiftMoEError("the weights' gradient needs the weights")
+    out = torch.empty((T, d), dtype=y.dtype, device=y.device)
+    dw = torch.empty((T, k), dtype=torch.float32, device=y.device) if x is not None else None
+    with _on(y.device):
+        L.check(L.load().smoe_unsort_rows(L.ptr(y), L.dtype_code(y.dtype), L.ptr(slot_row), L.ptr(w), T, k, d, rows_cap,
+                                          L.ptr(residual), L.ptr(out), L.ptr(x), L.ptr(dw),
+                                          L.stream_handle(y.device)), "smoe_unsort_rows")
+    return out if x is None else (out, dw)
+
+
+def _act_code(activation: str) -> int:
+    try:
+        return L.ACT_CODE[activation]
+    except (KeyError, TypeError):
+        raise L.SwiftMoEError(f"unknown activation {activation!r}: one of {', '.join(L.ACT_CODE)}") from None
+
+
+def _linear_dtype(t: torch.Tensor) -> int:
+    if t.dtype not in (torch.bfloat16, torch.float16):
+        raise L.SwiftMoEError(f"grouped linear layers are bf16 / fp16, got {t.dtype}")
+    return L.dtype_code(t.dtype)
+
+
+def _group_offsets(offsets: torch.Tensor, G: int):
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() != G + 1:
+        raise L.SwiftMoEError(f"offsets must be int32 [{G + 1}], got {offsets.dtype} {tuple(offsets.shape)}")
+
+
+def grouped_linear(A: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   activation: str = "none", residual: Optional[torch.Tensor] = None, *,
+                   preact: Optional[torch.Tensor] = None, w_layout: int = L.SMOE_W_NK,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """C[r] = act(A[r] W_g^T + bias[g]) + residual[r] for the rows r of group g, [offsets[g],
+    offsets[g+1]); W [G, N, K] (``L.SMOE_W_KN``: [G, K, N], C = A W_g), bias [G, N] in A's dtype
+    or fp32.  Rows of no group become the residual alone (zeros without one); given ``out``,
+    its rows of no group stay as they were.  ``preact`` [rows, N] receives A W_g^T + bias[g]."""
+    _need_cuda(A, W, offsets, bias, residual, preact, out)
+    _same_device(A.device, W, offsets, bias, residual, preact, out)
+    act, dt = _act_code(activation), _linear_dtype(A)
+    if A.dim() != 2 or W.dim() != 3 or W.dtype != A.dtype:
+        raise L.SwiftMoEError("A must be [rows, K], W [G, N, K] of the same dtype")
+    rows_cap, Kd = A.shape
+    G, N, K2 = W.shape if w_layout == L.SMOE_W_NK else (W.shape[0], W.shape[2], W.shape[1])
+    if K2 != Kd:
+        raise L.SwiftMoEError("K mismatch")
+    _group_offsets(offsets, G)
+    if bias is not None and (tuple(bias.shape) != (G, N) or bias.dtype not in (A.dtype, torch.float32)):
+        raise L.SwiftMoEError(f"bias must be {A.dtype} or float32 [{G}, {N}], got {bias.dtype} {tuple(bias.shape)}")
+    for name, t in (("residual", residual), ("preact", preact), ("out", out)):
+        if t is not None and (t.dtype != A.dtype or tuple(t.shape) != (rows_cap, N)):
+            raise L.SwiftMoEError(f"{name} must be {A.dtype} [{rows_cap}, {N}], got {t.dtype} {tuple(t.shape)}")
+    fill = out is None
+    if out is None:
+        out = torch.empty((rows_cap, N), dtype=A.dtype, device=A.device)
+    lib = L.load()
+    with _on(A.device):
+        need = lib.smoe_grouped_linear_workspace_size(rows_cap, N, w_layout)
+        ws = _workspace(A.device, need) if need else None
+        L.check(lib.smoe_grouped_linear(L.ptr(A), L.ptr(W), w_layout, L.ptr(bias),
+                                        L.dtype_code(bias.dtype) if bias is not None else dt, act, L.ptr(residual),
+                                        L.ptr(preact), int(fill), L.ptr(out), dt, L.ptr(offsets), G, rows_cap, N, Kd,
+                                        L.ptr(ws), need, L.stream_handle(A.device)), "smoe_grouped_linear")
+    return out
+
+
+def linear_act_bwd(dout: torch.Tensor, offsets: torch.Tensor, activation: str, preact: Optional[torch.Tensor] = None,
+                   bias_dtype: Optional[torch.dtype] = None):
+    """(dz, dbias): dz = dout * act'(preact) for the rows of the groups (dout itself for "none"),
+    dbias [G, N] = the groups' column sums of the unrounded dz, or None without bias_dtype."""
+    _need_cuda(dout, offsets, preact)
+    _same_device(dout.device, offsets, preact)
+    act, dt = _act_code(activation), _linear_dtype(dout)
+    rows_cap, N = dout.shape
+    G = offsets.numel() - 1
+    _group_offsets(offsets, G)
+    if act and (preact is None or preact.dtype != dout.dtype or preact.shape != dout.shape):
+        raise L.SwiftMoEError("preact must have dout's dtype and shape")
+    dz = torch.empty_like(dout) if act else dout
+    dbias = torch.empty((G, N), dtype=bias_dtype, device=dout.device) if bias_dtype is not None else None
+    lib = L.load()
+    with _on(dout.device):
+        need = lib.smoe_linear_act_bwd_workspace_size(rows_cap, N, G) if dbias is not None else 0
+        ws = _workspace(dout.device, need) if need else None
+        L.check(lib.smoe_linear_act_bwd(L.ptr(dout), L.ptr(preact), act, L.ptr(dz), L.ptr(dbias),
+                                        L.dtype_code(bias_dtype) if dbias is not None else dt, dt, L.ptr(offsets), G,
+                                        rows_cap, N, L.ptr(ws), need, L.stream_handle(dout.device)),
+                "smoe_linear_act_bwd")
+    return dz, dbias
+
+
+def linear_wgrad(dz: torch.Tensor, A: torch.Tensor, offsets: torch.Tensor,
+                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """dW [G, N, K] = dz_g^T A_g over the rows of every group (any group starts), in A's dtype
+    or fp32 (``out_dtype``); groups without rows get zeros."""
+    _need_cuda(dz, A, offsets)
+    _same_device(A.device, dz, offsets)
+    dt = _linear_dtype(A)
+    if dz.dtype != A.dtype or dz.dim() != 2 or A.dim() != 2 or dz.shape[0] != A.shape[0]:
+        raise L.SwiftMoEError("dz [rows, N] and A [rows, K] must have the same rows and dtype")
+    rows_cap, N = dz.shape
+    Kd, G = A.shape[1], offsets.numel() - 1
+    _group_offsets(offsets, G)
+    od = A.dtype if out_dtype is None else out_dtype
+    dW = torch.empty((G, N, Kd), dtype=od, device=A.device)
+    with _on(A.device):
+        L.check(L.load().smoe_linear_wgrad(L.ptr(dz), L.ptr(A), dt, L.ptr(offsets), G, rows_cap, N, Kd, L.ptr(dW),
+                                           L.dtype_code(od), L.stream_handle(A.device)), "smoe_linear_wgrad")
+    return dW
 
 
 def grouped_gemm(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor, *, B3: Optional[torch.Tensor] = None,

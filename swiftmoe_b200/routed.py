@@ -1,0 +1,140 @@
+"""The routed rows as differentiable operators: tokens sorted by expert, the experts'
+linear layers, and the rows back in token order.
+
+    rows, plan = sort_tokens(x, idx, num_experts)               # idx from kernels.router
+    h = grouped_linear(rows, w_in, plan["offsets"], bias=b_in, activation="gelu")
+    y = grouped_linear(h, w_out, plan["offsets"], bias=b_out)
+    out = unsort_tokens(y, plan, weights=w, residual=x)
+
+The layers (``StandardMoE`` / ``UltimateMoE``) run their own bias-free linear or SwiGLU
+experts in one call; these are the pieces for experts of another kind, with gradients.  No
+call waits for the device, and all of them can be captured into a CUDA graph, forward and
+backward.  (A backward captured while an eager graph of the same leaf tensors is alive
+accumulates into leaves whose stream torch recorded outside the capture, which torch does
+not allow; drop the eager graph's outputs before capturing, or call the ``kernels``
+functions that the backward consists of.)
+
+The reference's pieces are forward-only: models/ultimate_moe.py:118-125 (dispatch), 145-155
+(combine), 237-250 and models/baseline_moe.py:151-162 (experts).
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import kernels as K
+
+
+def _grads_wanted(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+class _SortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, plan):
+        ctx.plan = plan
+        ctx.save_for_backward(x if w is not None else None, w, plan["slot_row"])
+        return K.sort_rows(x, plan, w)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, drows):
+        x, w, _ = ctx.saved_tensors
+        drows = drows.contiguous()
+        if ctx.needs_input_grad[1]:
+            dx, dw = K.unsort_rows(drows, ctx.plan, w, x=x)
+            return dx, dw, None
+        return K.unsort_rows(drows, ctx.plan, w), None, None
+
+
+class _UnsortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, w, residual, plan):
+        ctx.plan, ctx.rows_cap = plan, rows.shape[0]
+        ctx.save_for_backward(rows if w is not None else None, w, plan["slot_row"])
+        return K.unsort_rows(rows, plan, w, residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        rows, w, _ = ctx.saved_tensors
+        need_rows, need_w, need_res, _ = ctx.needs_input_grad
+        dout = dout.contiguous()
+        drows = dw = None
+        if need_w:
+            drows, dw = K.sort_rows(dout, ctx.plan, w, rows_cap=ctx.rows_cap, y=rows)
+        elif need_rows:
+            drows = K.sort_rows(dout, ctx.plan, w, rows_cap=ctx.rows_cap)
+        return drows if need_rows else None, dw, dout if need_res else None, None
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, weight, bias, residual, offsets, activation):
+        keep = activation != "none" and any(ctx.needs_input_grad[:3])
+        z = torch.empty((a.shape[0], weight.shape[1]), dtype=a.dtype, device=a.device) if keep else None
+        out = K.grouped_linear(a, weight, offsets, bias, activation, residual, preact=z)
+        ctx.activation, ctx.bias_dtype = activation, bias.dtype if bias is not None else None
+        ctx.save_for_backward(a, weight, offsets, z)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        a, weight, offsets, z = ctx.saved_tensors
+        need_a, need_w, need_b, need_res = ctx.needs_input_grad[:4]
+        dout = dout.contiguous()
+        da = dw = db = None
+        if need_a or need_w or need_b:
+            dz, db = K.linear_act_bwd(dout, offsets, ctx.activation, z, ctx.bias_dtype if need_b else None)
+            if need_a:
+                da = K.grouped_linear(dz, weight, offsets, w_layout=L.SMOE_W_KN)
+            if need_w:
+                dw = K.linear_wgrad(dz, a, offsets)
+        return da, dw, db, dout if need_res else None, None, None
+
+
+def sort_tokens(x: torch.Tensor, idx: torch.Tensor, num_experts: int, weights: Optional[torch.Tensor] = None, *,
+                capacity: int = 0, row_align: int = 1) -> Tuple[torch.Tensor, dict]:
+    """(rows [R, d], plan): the tokens' rows grouped by expert, in (token, slot) order inside
+    an expert, and the dispatch plan (``kernels.dispatch_plan``; ``plan["offsets"]`` [E+1]
+    are the experts' row ranges, ``plan["counts"]`` the rows routed to each).
+
+    x [T, d] fp32 / fp16 / bf16; idx [T, k] int32 expert of every slot, -1 for none (k <=
+    32); weights [T, k] fp32 multiplies the rows (default: rows are copies).  At most
+    ``capacity`` rows per expert are kept (0: all), group starts are multiples of
+    ``row_align``.  R is the plan's upper bound on the rows; rows of no slot are zero.
+    Differentiable in x and weights."""
+    plan = K.dispatch_plan(idx, num_experts, capacity, row_align)
+    if _grads_wanted(x, weights):
+        return _SortTokens.apply(x, weights, plan), plan
+    return K.sort_rows(x, plan, weights), plan
+
+
+def unsort_tokens(rows: torch.Tensor, plan: dict, weights: Optional[torch.Tensor] = None,
+                  residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out [T, d]: the rows of every token summed in slot order, each times its weight
+    (``weights`` [T, k] fp32, default 1), plus ``residual`` [T, d].  Dropped slots add
+    nothing.  fp32 sums, one rounding.  Differentiable in rows, weights and residual."""
+    if _grads_wanted(rows, weights, residual):
+        return _UnsortTokens.apply(rows, weights, residual, plan)
+    return K.unsort_rows(rows, plan, weights, residual)
+
+
+def grouped_linear(a: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   activation: str = "none", residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out [R, N] = act(a W_g^T + bias[g]) + residual for the rows [offsets[g], offsets[g+1]) of
+    every group g; rows of no group are the residual alone (zeros without one).
+
+    a [R, K] and weight [G, N, K] bf16 / fp16, K and N multiples of 8; offsets [G+1] int32 on
+    the device (``plan["offsets"]``; groups may start anywhere); bias [G, N] in a's dtype or
+    fp32; activation "none", "relu", "gelu" (exact), "gelu_tanh" or "silu"; residual [R, N].
+    fp32 accumulation, one rounding.  Differentiable in a, weight, bias and residual; the
+    backward keeps the pre-activations, rounded to a's dtype, from the forward."""
+    K._act_code(activation)
+    if _grads_wanted(a, weight, bias, residual):
+        return _GroupedLinear.apply(a, weight, bias, residual, offsets, activation)
+    return K.grouped_linear(a, weight, offsets, bias, activation, residual)

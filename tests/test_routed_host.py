@@ -1,0 +1,81 @@
+"""Refusals of the routed-row entry points that need no GPU."""
+import pytest
+import torch
+
+import swiftmoe_b200 as S
+from swiftmoe_b200 import _lib as L
+from swiftmoe_b200 import build
+from swiftmoe_b200._lib import SwiftMoEError
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return L.load()
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(4, 16).bfloat16()
+    idx = torch.zeros((4, 2), dtype=torch.int32)
+    plan = dict(counts=idx[0], offsets=idx[0], slot_row=idx.view(-1), row_token=idx.view(-1), rows_cap=8, T=4, k=2)
+    w = torch.randn(2, 8, 16).bfloat16()
+    off = torch.tensor([0, 2, 4], dtype=torch.int32)
+    for call in (lambda: S.sort_tokens(x, idx, 2), lambda: S.unsort_tokens(x, plan),
+                 lambda: S.grouped_linear(x, w, off), lambda: S.grouped_linear(x, w, off, activation="swish")):
+        with pytest.raises(SwiftMoEError):
+            call()
+
+
+BF, F32, P = 2, 0, 4096   # P: a non-null, aligned address that is never used
+
+
+def test_sort_and_unsort_refusals(lib):
+    sort = lambda **a: lib.smoe_sort_rows(*{**dict(x=P, dt=BF, sr=P, w=None, T=4, k=2, d=8, rt=None, off=P, E=2, cap=8,  # noqa: E731
+                                                   rows=P, y=None, dw=None, st=None), **a}.values())
+    for bad in (dict(dt=7), dict(T=-1), dict(k=0), dict(d=0), dict(E=0), dict(cap=-1), dict(x=None), dict(sr=None),
+                dict(off=None), dict(rows=None), dict(dw=P, w=P), dict(dw=P, y=P)):
+        assert sort(**bad) == -1, bad
+    assert sort(k=33) == -4 and sort(cap=1 << 31) == -4
+    assert sort(T=0, cap=0) == 0
+    un = lambda **a: lib.smoe_unsort_rows(*{**dict(y=P, dt=BF, sr=P, w=None, T=4, k=2, d=8, cap=8, res=None, out=P, x=None,  # noqa: E731
+                                                   dw=None, st=None), **a}.values())
+    for bad in (dict(dt=7), dict(T=-1), dict(k=0), dict(d=0), dict(cap=-1), dict(y=None), dict(sr=None), dict(out=None),
+                dict(dw=P, w=P), dict(dw=P, x=P)):
+        assert un(**bad) == -1, bad
+    assert un(k=33) == -4 and un(T=0) == 0
+
+
+def test_linear_refusals(lib):
+    lin = lambda **a: lib.smoe_grouped_linear(*{**dict(A=P, W=P, lay=0, b=None, bdt=BF, act=0, res=None, z=None, fill=1, C=P,  # noqa: E731
+                                                       dt=BF, off=P, G=2, R=300, N=16, K=16, ws=None, wsb=0, st=None), **a}.values())
+    for bad in (dict(G=0), dict(N=0), dict(K=0), dict(R=-1), dict(act=5), dict(act=-1), dict(lay=2), dict(A=None),
+                dict(W=None), dict(C=None), dict(off=None)):
+        assert lin(**bad) == -1, bad
+    for bad in (dict(dt=F32), dict(b=P, bdt=1), dict(N=12), dict(K=12), dict(G=1025), dict(R=1 << 31), dict(A=P + 2),
+                dict(W=P + 8), dict(C=P + 4), dict(b=P + 2), dict(res=P + 2), dict(z=P + 2)):
+        assert lin(**bad) == -4, bad
+    assert lin(R=0) == 0
+    act = lambda **a: lib.smoe_linear_act_bwd(*{**dict(dout=P, z=P, act=2, dz=P, db=None, bdt=BF, dt=BF, off=P, G=2, R=30, N=16,  # noqa: E731
+                                                       ws=None, wsb=0, st=None), **a}.values())
+    for bad in (dict(G=0), dict(N=0), dict(R=-1), dict(act=5), dict(dout=None), dict(z=None), dict(dz=None), dict(off=None)):
+        assert act(**bad) == -1, bad
+    for bad in (dict(dt=F32), dict(db=P, bdt=1), dict(N=12), dict(G=1025), dict(dout=P + 2), dict(z=P + 2), dict(dz=P + 2)):
+        assert act(**bad) == -4, bad
+    assert act(db=P) == -5 and act(R=0) == 0 and act(act=0) == 0
+    wg = lambda **a: lib.smoe_linear_wgrad(*{**dict(dz=P, A=P, dt=BF, off=P, G=2, R=30, N=16, K=16, dW=P, odt=BF, st=None),  # noqa: E731
+                                             **a}.values())
+    for bad in (dict(G=0), dict(N=0), dict(K=0), dict(R=-1), dict(dz=None), dict(A=None), dict(off=None), dict(dW=None)):
+        assert wg(**bad) == -1, bad
+    for bad in (dict(dt=F32), dict(odt=1), dict(N=12), dict(K=12), dict(G=1025), dict(dz=P + 2), dict(A=P + 2), dict(dW=P + 2)):
+        assert wg(**bad) == -4, bad
+
+
+def test_workspace_sizes(lib):
+    # split-K scratch only where the launch can have few tiles
+    assert lib.smoe_grouped_linear_workspace_size(2, 4096, L.SMOE_W_NK) == 0       # decode kernel
+    assert lib.smoe_grouped_linear_workspace_size(2, 4096, L.SMOE_W_KN) > 0
+    assert lib.smoe_grouped_linear_workspace_size(64, 4096, L.SMOE_W_NK) > 0
+    assert lib.smoe_grouped_linear_workspace_size(16384, 4096, L.SMOE_W_NK) == 0
+    # bias partials: at most 64 slices of at least 64 rows, plus one row per group
+    assert lib.smoe_linear_act_bwd_workspace_size(64, 8, 4) == (1 + 4) * 8 * 4
+    assert lib.smoe_linear_act_bwd_workspace_size(1 << 20, 8, 4) == (64 + 4) * 8 * 4
