@@ -72,6 +72,8 @@ SIGNATURES = {
     "smoe_permute_rows": (_i32, [_vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _vp, _vp]),
     "smoe_combine": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
     "smoe_sort_rows": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _vp, _vp, _vp, _vp]),
+    "smoe_sort_tokens": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp,
+                                _vp, _sz, _vp]),
     "smoe_unsort_rows": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp]),
     "smoe_grouped_linear_workspace_size": (_sz, [_i64, _i32, _i32]),
     "smoe_grouped_linear": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _i32, _i64, _i32,
@@ -128,6 +130,8 @@ class SwiftMoEError(RuntimeError):
 def load() -> C.CDLL:
     """Load libswiftmoe.so (raises if it has not been built)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not LIB_PATH.exists():
@@ -139,7 +143,7 @@ def load() -> C.CDLL:
                 fn = getattr(lib, name)
                 fn.restype = res
                 fn.argtypes = args
-            _lib = lib
+            _lib = lib   # complete: other threads take it without the lock
     return _lib
 
 
@@ -156,7 +160,12 @@ def ptr(t) -> int | None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the handle alone: current_stream() also makes a Stream object, 2.5 us of a call's
+    # host time
+    index = device.index if isinstance(device, torch.device) else None
+    if index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -1091,6 +1091,22 @@ int smoe_sort_rows(const void* x, int dtype, const int32_t* slot_row, const floa
   return SMOE_OK;
 }
 
+int smoe_sort_tokens(const void* x, int dtype, const int32_t* idx, const float* w, int T, int k, int d, int E,
+                     int capacity, int row_align, int32_t* expert_counts, int32_t* expert_offsets, int32_t* slot_row,
+                     int32_t* row_token, int64_t rows_cap, void* rows, void* workspace, size_t workspace_bytes,
+                     smoe_stream_t stream) {
+  // everything the second call refuses, before the first one launches
+  if (elt_size(dtype) == 0 || d < 1 || (T > 0 && !x) || (rows_cap > 0 && !rows)) return SMOE_ERR_INVALID;
+  if (k > rows::MAX_K || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  // decode: the row copy is scheduled while the one-block plan finishes
+  const PdlScope pdl(T >= 0 && (int64_t)T * k <= kPlanChunk);
+  const int rc = smoe_dispatch_plan(idx, T, k, E, capacity, row_align, expert_counts, expert_offsets, slot_row, row_token,
+                                    std::max<int64_t>(rows_cap, 1), workspace, workspace_bytes, stream);
+  if (rc) return rc;
+  return smoe_sort_rows(x, dtype, slot_row, w, T, k, d, row_align > 1 ? row_token : nullptr, expert_offsets, E, rows_cap,
+                        rows, nullptr, nullptr, stream);
+}
+
 int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const float* w, int T, int k, int d,
                      int64_t rows_cap, const void* residual, void* out, const void* x, float* dw,
                      smoe_stream_t stream) {

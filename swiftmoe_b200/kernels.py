@@ -31,10 +31,13 @@ def _same_device(device, *ts):
             raise L.SwiftMoEError(f"tensors on different devices: {device} and {t.device}")
 
 
+_HERE = nullcontext()
+
+
 def _on(device):
     """The device the launch belongs to, made current if it is not (streams and tensors of
     another GPU than the current one)."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def router(x: torch.Tensor, gate_w: torch.Tensor, k: int, logit_bias: Optional[torch.Tensor] = None,
@@ -167,6 +170,37 @@ def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, 
                                         L.ptr(row_token), L.ptr(plan["offsets"]), plan["offsets"].numel() - 1, rows_cap,
                                         L.ptr(rows), L.ptr(y), L.ptr(dw), L.stream_handle(x.device)), "smoe_sort_rows")
     return rows if y is None else (rows, dw)
+
+
+def sort_tokens(x: torch.Tensor, idx: torch.Tensor, num_experts: int, w: Optional[torch.Tensor] = None,
+                capacity: int = 0, row_align: int = 1):
+    """(rows, plan): ``dispatch_plan`` and ``sort_rows`` in one library call."""
+    _need_cuda(x, idx, w)
+    dev = x.device
+    _same_device(dev, idx, w)
+    if idx.dtype != torch.int32 or idx.dim() != 2:
+        raise L.SwiftMoEError("idx must be int32 [T, k]")
+    T, k = idx.shape
+    if x.dim() != 2 or x.shape[0] != T:
+        raise L.SwiftMoEError(f"idx is for {T} tokens, got x of shape {tuple(x.shape)}")
+    if w is not None and (w.dtype != torch.float32 or w.shape != idx.shape):
+        raise L.SwiftMoEError(f"weights must be float32 [{T}, {k}], got {w.dtype} {tuple(w.shape)}")
+    dt, d, E, lib, i32 = L.dtype_code(x.dtype), x.shape[1], num_experts, L.load(), torch.int32
+    rows_cap = lib.smoe_plan_rows_cap(T, k, E, capacity, row_align)
+    need = lib.smoe_plan_workspace_size(T, k, E)
+    counts = torch.empty(max(E, 0), dtype=i32, device=dev)
+    offsets = torch.empty(max(E, 0) + 1, dtype=i32, device=dev)
+    slot_row = torch.empty(T * k, dtype=i32, device=dev)
+    row_token = torch.empty(max(rows_cap, 1), dtype=i32, device=dev)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    rows = torch.empty((rows_cap, d), dtype=x.dtype, device=dev)
+    with _on(dev):
+        L.check(lib.smoe_sort_tokens(x.data_ptr(), dt, idx.data_ptr(), L.ptr(w), T, k, d, E, capacity, row_align,
+                                     counts.data_ptr(), offsets.data_ptr(), slot_row.data_ptr(), row_token.data_ptr(),
+                                     rows_cap, rows.data_ptr(), ws.data_ptr(), need, L.stream_handle(dev)),
+                "smoe_sort_tokens")
+    return rows, dict(counts=counts, offsets=offsets, slot_row=slot_row, row_token=row_token, rows_cap=rows_cap, T=T,
+                      k=k, row_align=row_align)
 
 
 def unsort_rows(y: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,

@@ -34,10 +34,12 @@ def _grads_wanted(*ts) -> bool:
 
 class _SortTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, plan):
+    def forward(ctx, x, w, args, made):
+        rows, plan = K.sort_tokens(x, args[0], args[1], w, args[2], args[3])
+        made.append(plan)
         ctx.plan = plan
         ctx.save_for_backward(x if w is not None else None, w, plan["slot_row"])
-        return K.sort_rows(x, plan, w)
+        return rows
 
     @staticmethod
     @once_differentiable
@@ -46,8 +48,8 @@ class _SortTokens(torch.autograd.Function):
         drows = drows.contiguous()
         if ctx.needs_input_grad[1]:
             dx, dw = K.unsort_rows(drows, ctx.plan, w, x=x)
-            return dx, dw, None
-        return K.unsort_rows(drows, ctx.plan, w), None, None
+            return dx, dw, None, None
+        return K.unsort_rows(drows, ctx.plan, w), None, None, None
 
 
 class _UnsortTokens(torch.autograd.Function):
@@ -108,10 +110,11 @@ def sort_tokens(x: torch.Tensor, idx: torch.Tensor, num_experts: int, weights: O
     ``capacity`` rows per expert are kept (0: all), group starts are multiples of
     ``row_align``.  R is the plan's upper bound on the rows; rows of no slot are zero.
     Differentiable in x and weights."""
-    plan = K.dispatch_plan(idx, num_experts, capacity, row_align)
     if _grads_wanted(x, weights):
-        return _SortTokens.apply(x, weights, plan), plan
-    return K.sort_rows(x, plan, weights), plan
+        made = []
+        rows = _SortTokens.apply(x, weights, (idx, num_experts, capacity, row_align), made)
+        return rows, made[0]
+    return K.sort_tokens(x, idx, num_experts, weights, capacity, row_align)
 
 
 def unsort_tokens(rows: torch.Tensor, plan: dict, weights: Optional[torch.Tensor] = None,

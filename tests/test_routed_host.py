@@ -45,6 +45,15 @@ def test_sort_and_unsort_refusals(lib):
     assert un(k=33) == -4 and un(T=0) == 0
 
 
+def test_sort_tokens_refusals(lib):
+    st = lambda **a: lib.smoe_sort_tokens(*{**dict(x=P, dt=BF, idx=P, w=None, T=4, k=2, d=8, E=3, cap=0, al=1, cnt=P, off=P,  # noqa: E731
+                                                   sr=P, rt=P, rows_cap=8, rows=P, ws=P, wsb=1 << 20, st=None), **a}.values())
+    for bad in (dict(dt=7), dict(T=-1), dict(k=0), dict(d=0), dict(E=0), dict(al=0), dict(x=None), dict(idx=None),
+                dict(cnt=None), dict(off=None), dict(sr=None), dict(rt=None), dict(rows=None), dict(rows_cap=7)):
+        assert st(**bad) == -1, bad
+    assert st(k=33) == -4 and st(ws=None) == -5 and st(wsb=8) == -5
+
+
 def test_linear_refusals(lib):
     lin = lambda **a: lib.smoe_grouped_linear(*{**dict(A=P, W=P, lay=0, b=None, bdt=BF, act=0, res=None, z=None, fill=1, C=P,  # noqa: E731
                                                        dt=BF, off=P, G=2, R=300, N=16, K=16, ws=None, wsb=0, st=None), **a}.values())
