@@ -666,24 +666,31 @@ cudaError_t launch_act_bwd(const void* dout, const void* z, void* dz, int act, c
 }
 
 // ------------------------------------------------------------------ tokens <-> rows
-// One warp per token, or, for batches of fewer tokens than would fill the GPU that way,
-// the eight warps of a block.
-int token_warps(int T) { return T <= 4 * device_sms() ? 8 : 1; }
-unsigned token_grid(int T, int wpt) {
-  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv((int64_t)T * wpt, rows::WARPS), (int64_t)device_sms() * 8));
+// One warp per token, or the eight warps of a block for few tokens with long rows.  Sort with
+// gradient of the weights / unsort, one warp against eight: 6.9 / 8.2 against 7.3 / 5.2 us
+// for 1000 x 2 bf16 rows of 4096, 9.3 / 10.0 against 12.5 / 8.5 for 2000, 10.4 / 14.0 against
+// 9.9 / 8.0 for 1537 x 3 fp32 rows of 1027 single elements, 6.6 / 3.5 against 12.9 / 8.8 for
+// 4000 x 2 rows of 64 pieces.
+int token_warps(int T, int64_t pieces) { return T < 12 * device_sms() && pieces >= 128 ? 8 : 1; }
+// waves: blocks per SM at most.  sort hands its tokens to 64 (222 us with 8, 193 with 64 for
+// 32768 x 8 fp16 rows of 2048: short blocks even out the end), unsort keeps 8 resident ones.
+unsigned token_grid(int T, int wpt, int waves) {
+  return (unsigned)std::max<int64_t>(
+      1, std::min<int64_t>(cdiv((int64_t)T * wpt, rows::WARPS), (int64_t)device_sms() * waves));
 }
 
 template <typename T, int VEC, int WPT>
 cudaError_t launch_sort_rows(const void* x, const int32_t* sr, const float* w, int T_, int k, int d,
                              const int32_t* row_token, const int32_t* offsets, int E, int64_t rows_cap, void* out,
                              const void* y, float* dw, cudaStream_t st) {
-  const unsigned grid = token_grid(T_, WPT);
+  const unsigned grid = token_grid(T_, WPT, 64);
 #define SMOE_SORT(HW, DOT)                                                                                          \
   return launch_k(rows::sort_rows_kernel<T, VEC, WPT, HW, DOT>, grid, rows::THREADS, 0, st, (const T*)x, sr, w, T_, k, \
                   d, row_token, offsets, E, rows_cap, (T*)out, (const T*)y, dw)
-  if (dw) SMOE_SORT(true, true);
-  if (w) SMOE_SORT(true, false);
-  SMOE_SORT(false, false);
+  if (dw && k <= 8) SMOE_SORT(true, 8);
+  if (dw) SMOE_SORT(true, rows::MAX_K);
+  if (w) SMOE_SORT(true, 0);
+  SMOE_SORT(false, 0);
 #undef SMOE_SORT
 }
 
@@ -691,7 +698,7 @@ template <typename T, int VEC, int WPT>
 cudaError_t launch_unsort_rows(const void* y, const int32_t* sr, const float* w, int T_, int k, int d,
                                int64_t rows_cap, const void* residual, void* out, const void* x, float* dw,
                                cudaStream_t st) {
-  const unsigned grid = token_grid(T_, WPT);
+  const unsigned grid = token_grid(T_, WPT, 8);
 #define SMOE_UNSORT(HW, DOT)                                                                                      \
   return launch_k(rows::unsort_rows_kernel<T, VEC, WPT, HW, DOT>, grid, rows::THREADS, 0, st, (const T*)y, sr, w, T_, \
                   k, d, rows_cap, (const T*)residual, (T*)out, (const T*)x, dw)
@@ -941,10 +948,12 @@ int smoe_topk_from_logits(const float* logits, int T, int E, int k, int32_t* idx
 }
 
 // ------------------------------------------------------------------ dispatch plan
+constexpr int kPlanMaxBlocks = 148;  // of a plan of several blocks (one per SM)
+
 size_t smoe_plan_workspace_size(int T, int k, int E) {
   if (T < 0 || k < 1 || E < 1) return 0;
-  const int64_t nb = std::max<int64_t>(1, cdiv((int64_t)T * k, kPlanChunk));
-  return 2 * align_up((size_t)nb * E * sizeof(int32_t), 256);
+  const int64_t nb = std::max<int64_t>(std::min<int64_t>(kPlanMaxBlocks, cdiv((int64_t)T * k, kPlanThreads)), 1);
+  return align_up((size_t)nb * E * sizeof(int32_t), 256);
 }
 
 int64_t smoe_plan_rows_cap(int T, int k, int E, int capacity, int row_align) {
@@ -966,12 +975,8 @@ int smoe_dispatch_plan(const int32_t* idx, int T, int k, int E, int capacity, in
   if (!workspace || workspace_bytes < need) return SMOE_ERR_WORKSPACE;
   const int64_t n_slots = (int64_t)T * k;
   if (n_slots > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
-  const int nb = (int)std::max<int64_t>(1, cdiv(n_slots, kPlanChunk));
-  int32_t* hist = static_cast<int32_t*>(workspace);
-  int32_t* base = reinterpret_cast<int32_t*>(static_cast<unsigned char*>(workspace) +
-                                             align_up((size_t)nb * E * sizeof(int32_t), 256));
   const int smem_w = kPlanWarps * E * (int)sizeof(int);
-  if (nb == 1) {  // one block: count, scan and scatter in one launch
+  if (n_slots <= kPlanChunk) {  // one block: count, scan and scatter in one launch
     static SmemGrant done_1;
     const int smem_1 = smem_w + (E + 1) * (int)sizeof(int);
     SMOE_CK(ensure_smem(plan_small_kernel, smem_1, &done_1));
@@ -980,19 +985,24 @@ int smoe_dispatch_plan(const int32_t* idx, int T, int k, int E, int capacity, in
     SMOE_CK(cudaGetLastError());
     return SMOE_OK;
   }
-  static SmemGrant done_c, done_s;
-  SMOE_CK(ensure_smem(plan_count_kernel, smem_w, &done_c));
-  SMOE_CK(ensure_smem(plan_scatter_kernel, smem_w, &done_s));
-  SMOE_CK(launch_k(plan_count_kernel, nb, kPlanThreads, smem_w, st, idx, n_slots, E, hist));
+  int32_t* hist = static_cast<int32_t*>(workspace);
+  // 32 warps per block once eight of them would take more than two steps of 32 slots each
+  // (their counters fit in shared memory up to 512 experts).  This plan / the former
+  // count, scan and scatter launches, back to back: 6.2 / 12.8 us for 32768 slots of 8
+  // experts, 9.0 / 17.3 for 32768 of 128, 14.9 / 23.3 for 262144 of 128.
+  const int threads = E <= 512 && n_slots > (int64_t)2 * kPlanMaxBlocks * kPlanThreads ? 32 * kPlanBigWarps : kPlanThreads;
+  const int steps = (int)cdiv(n_slots, (int64_t)kPlanMaxBlocks * threads);  // of 32 slots per warp
+  const int nb = (int)cdiv(n_slots, (int64_t)steps * threads);
+  const int smem_h = threads / 32 * E * (int)sizeof(int);
+  static SmemGrant done_h, done_p;
+  const int smem_p = smem_h + (3 * E + 1) * (int)sizeof(int);
+  SMOE_CK(ensure_smem(plan_hist_kernel, smem_h, &done_h));
+  SMOE_CK(ensure_smem(plan_place_kernel, smem_p, &done_p));
+  SMOE_CK(launch_k(plan_hist_kernel, nb, threads, smem_h, st, idx, n_slots, E, steps, hist));
   SMOE_CK(cudaGetLastError());
-  SMOE_CK(launch_k(plan_scan_kernel, 1, 1024, E * sizeof(int), st, hist, nb, E, capacity, row_align, base, expert_counts,
-                                                     expert_offsets, row_token));
+  SMOE_CK(launch_k(plan_place_kernel, nb, threads, smem_p, st, idx, n_slots, k, E, capacity, row_align, steps, hist,
+                   expert_counts, expert_offsets, slot_row, row_token));
   SMOE_CK(cudaGetLastError());
-  if (n_slots > 0) {
-    SMOE_CK(launch_k(plan_scatter_kernel, nb, kPlanThreads, smem_w, st, idx, n_slots, k, E, capacity, base, expert_offsets,
-                                                          slot_row, row_token));
-    SMOE_CK(cudaGetLastError());
-  }
   return SMOE_OK;
 }
 
@@ -1081,7 +1091,7 @@ int smoe_sort_rows(const void* x, int dtype, const int32_t* slot_row, const floa
   if (T == 0 && rows_cap == 0) return SMOE_OK;
   if (!expert_offsets || (rows_cap > 0 && !rows) || (T > 0 && (!x || !slot_row)) || (dw && (!w || (rows_cap > 0 && !y))))
     return SMOE_ERR_INVALID;
-  const int vec = row_vec(es, d, {x, rows, dw ? y : nullptr}), wpt = token_warps(T);
+  const int vec = row_vec(es, d, {x, rows, dw ? y : nullptr}), wpt = token_warps(T, d / vec);
   cudaStream_t st = (cudaStream_t)stream;
 #define SMOE_ROWS_LAUNCH(TY, VV, WW) \
   (launch_sort_rows<TY, VV, WW>(x, slot_row, w, T, k, d, row_token, expert_offsets, E, rows_cap, rows, y, dw, st))
@@ -1098,8 +1108,8 @@ int smoe_sort_tokens(const void* x, int dtype, const int32_t* idx, const float* 
   // everything the second call refuses, before the first one launches
   if (elt_size(dtype) == 0 || d < 1 || (T > 0 && !x) || (rows_cap > 0 && !rows)) return SMOE_ERR_INVALID;
   if (k > rows::MAX_K || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
-  // decode: the row copy is scheduled while the one-block plan finishes
-  const PdlScope pdl(T >= 0 && (int64_t)T * k <= kPlanChunk);
+  // each launch is scheduled while its short predecessor finishes
+  const PdlScope pdl(true);
   const int rc = smoe_dispatch_plan(idx, T, k, E, capacity, row_align, expert_counts, expert_offsets, slot_row, row_token,
                                     std::max<int64_t>(rows_cap, 1), workspace, workspace_bytes, stream);
   if (rc) return rc;
@@ -1115,7 +1125,7 @@ int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const fl
   if (k > rows::MAX_K || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
   if (T == 0) return SMOE_OK;
   if (!slot_row || !out || (rows_cap > 0 && !y) || (dw && (!w || !x))) return SMOE_ERR_INVALID;
-  const int vec = row_vec(es, d, {y, out, residual, dw ? x : nullptr}), wpt = token_warps(T);
+  const int vec = row_vec(es, d, {y, out, residual, dw ? x : nullptr}), wpt = token_warps(T, d / vec);
   cudaStream_t st = (cudaStream_t)stream;
 #define SMOE_ROWS_LAUNCH(TY, VV, WW) \
   (launch_unsort_rows<TY, VV, WW>(y, slot_row, w, T, k, d, rows_cap, residual, out, x, dw, st))

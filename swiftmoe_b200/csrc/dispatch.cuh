@@ -19,19 +19,19 @@ constexpr int kPlanChunk = kPlanWarps * kPlanSlotsPerWarp;  // slots per block
 
 // Per-warp counts of each expert over the warp's slot range; cnt is [kPlanWarps][E].
 __device__ __forceinline__ void plan_warp_counts(const int32_t* __restrict__ idx, int64_t n_slots, int E,
-                                                 int64_t slot0, int* cnt) {
+                                                 int64_t slot0, int* cnt, int steps = kPlanSlotsPerWarp / 32) {
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
   int* my = cnt + warp * E;
-  for (int step = 0; step < kPlanSlotsPerWarp / 32; ++step) {
-    const int64_t s = slot0 + warp * kPlanSlotsPerWarp + step * 32 + lane;
-    int e = -1;
-    if (s < n_slots) {
-      e = idx[s];
-      if (e != -1 && (e < 0 || e >= E)) {  // -1 marks a slot to skip
-        set_device_error(kErrBadExpertIndex);
-        e = -1;
-      }
+  const int64_t s0 = slot0 + (int64_t)warp * steps * 32 + lane;
+  int next = s0 < n_slots ? idx[s0] : -1;
+  for (int step = 0; step < steps; ++step) {
+    const int64_t s = s0 + step * 32;
+    int e = next;
+    next = step + 1 < steps && s + 32 < n_slots ? idx[s + 32] : -1;  // on its way during this step
+    if (e != -1 && (e < 0 || e >= E)) {  // -1 marks a slot to skip
+      set_device_error(kErrBadExpertIndex);
+      e = -1;
     }
     const unsigned peers = __match_any_sync(0xffffffffu, e);
     if (e >= 0 && lane == __ffs(peers) - 1) my[e] += __popc(peers);
@@ -172,6 +172,118 @@ __global__ void __launch_bounds__(kPlanThreads) plan_scatter_kernel(const int32_
   }
 }
 
+// The plan of more than one block in two launches, the scan without a kernel of its own:
+// hist[b][e] from plan_hist_kernel, then every block of plan_place_kernel adds up the
+// columns of hist itself -- all blocks for the experts' totals, the blocks before it for its
+// base -- and scans the kept totals in shared memory.  The launch has at most about one
+// block per SM (`steps` 32-slot steps per warp, 8 or 32 warps), so hist is at most
+// 148 x E and each block reads it from L2 in a few microseconds, less than a third launch
+// with one block.  Same arrays as plan_count -> plan_scan -> plan_scatter.
+constexpr int kPlanBigWarps = 32;  // per block, for many slots of few experts
+
+__global__ void __launch_bounds__(32 * kPlanBigWarps) plan_hist_kernel(const int32_t* __restrict__ idx, int64_t n_slots,
+                                                                 int E, int steps, int32_t* __restrict__ hist) {
+  pdl_wait_and_release();
+  extern __shared__ int cnt[];  // [warps][E]
+  const int warps = blockDim.x >> 5;
+  for (int i = threadIdx.x; i < warps * E; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  plan_warp_counts(idx, n_slots, E, (int64_t)blockIdx.x * steps * blockDim.x, cnt, steps);
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += blockDim.x) {
+    int s = 0;
+#pragma unroll 8
+    for (int w = 0; w < warps; ++w) s += cnt[w * E + e];
+    hist[(size_t)blockIdx.x * E + e] = s;
+  }
+}
+
+__device__ int block_exclusive_scan(int* data, int n, int* scratch);
+
+__global__ void __launch_bounds__(32 * kPlanBigWarps)
+    plan_place_kernel(const int32_t* __restrict__ idx, int64_t n_slots, int k, int E, int capacity, int row_align,
+                      int steps, const int32_t* __restrict__ hist, int32_t* __restrict__ counts,
+                      int32_t* __restrict__ offsets, int32_t* __restrict__ slot_row, int32_t* __restrict__ row_token) {
+  pdl_wait_and_release();
+  extern __shared__ int sm_plan[];
+  int* cnt = sm_plan;                 // [warps][E]: counts, then running positions
+  const int warps = blockDim.x >> 5, nt = blockDim.x;
+  int* s_tot = cnt + warps * E;  // [E] rows of the expert
+  int* s_bef = s_tot + E;             // [E] rows in the blocks before this one
+  int* s_off = s_bef + E;             // [E + 1] first row
+  __shared__ int scratch[32];
+  for (int i = threadIdx.x; i < (warps + 2) * E; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  plan_warp_counts(idx, n_slots, E, (int64_t)blockIdx.x * steps * blockDim.x, cnt, steps);
+  const int parts = E < nt ? nt / E : 1;  // threads that share a column
+  const int part = E < nt ? (int)threadIdx.x / E : 0;
+  if (part < parts)
+    for (int e = E < nt ? (int)threadIdx.x % E : (int)threadIdx.x; e < E; e += nt) {
+      int tot = 0, bef = 0;
+#pragma unroll 8
+      for (int b = part; b < (int)gridDim.x; b += parts) {
+        const int v = hist[(size_t)b * E + e];
+        tot += v;
+        if (b < (int)blockIdx.x) bef += v;
+      }
+      atomicAdd(s_tot + e, tot);
+      atomicAdd(s_bef + e, bef);
+    }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += blockDim.x) {
+    const int kept = capacity > 0 ? min(s_tot[e], capacity) : s_tot[e];
+    s_off[e] = (kept + row_align - 1) / row_align * row_align;
+    int run = s_bef[e];
+#pragma unroll 8
+    for (int w = 0; w < warps; ++w) {
+      const int c = cnt[w * E + e];
+      cnt[w * E + e] = run;
+      run += c;
+    }
+  }
+  __syncthreads();
+  const int total = block_exclusive_scan(s_off, E, scratch);
+  if (blockIdx.x == 0) {
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+      counts[e] = s_tot[e];
+      offsets[e] = s_off[e];
+      if (row_align > 1) {  // alignment padding rows carry token -1
+        const int kept = capacity > 0 ? min(s_tot[e], capacity) : s_tot[e];
+        const int stop = e + 1 < E ? s_off[e + 1] : total;
+        for (int r = s_off[e] + kept; r < stop; ++r) row_token[r] = -1;
+      }
+    }
+    if (threadIdx.x == 0) offsets[E] = total;
+  }
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  int* pos = cnt + warp * E;
+  const unsigned lt = (1u << lane) - 1u;
+  const int64_t s0 = (int64_t)blockIdx.x * steps * blockDim.x + (int64_t)warp * steps * 32 + lane;
+  int next = s0 < n_slots ? idx[s0] : -1;
+  for (int step = 0; step < steps; ++step) {
+    const int64_t s = s0 + step * 32;
+    int e = next;
+    next = step + 1 < steps && s + 32 < n_slots ? idx[s + 32] : -1;
+    if (e < 0 || e >= E) e = -1;
+    const unsigned peers = __match_any_sync(0xffffffffu, e);
+    int p = 0;
+    if (e >= 0) p = pos[e] + __popc(peers & lt);
+    __syncwarp();
+    if (e >= 0 && lane == __ffs(peers) - 1) pos[e] += __popc(peers);
+    __syncwarp();
+    if (s < n_slots) {
+      if (e < 0 || (capacity > 0 && p >= capacity)) {
+        slot_row[s] = -1;
+      } else {
+        const int row = s_off[e] + p;
+        slot_row[s] = row;
+        row_token[row] = (int32_t)(s / k);
+      }
+    }
+  }
+}
+
 // The three plan kernels in one launch for plans of one block (n_slots <= kPlanChunk,
 // decode-sized batches): the single block's base is 0 for every expert, so counting,
 // the capacity cut, the scan and the stable scatter run back to back in shared memory
@@ -189,7 +301,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_small_kernel(const int32_t*
   __shared__ int s_warp[kPlanWarps];
   for (int i = threadIdx.x; i < kPlanWarps * E; i += blockDim.x) cnt[i] = 0;
   __syncthreads();
-  plan_warp_counts(idx, n_slots, E, 0, cnt);
+  const int steps = (int)((n_slots + kPlanThreads - 1) / kPlanThreads);  // of 32 slots per warp
+  plan_warp_counts(idx, n_slots, E, 0, cnt, steps);
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
     int run = 0;
@@ -240,8 +353,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_small_kernel(const int32_t*
   }
   int* pos = cnt + warp * E;
   const unsigned lt = (1u << lane) - 1u;
-  for (int step = 0; step < kPlanSlotsPerWarp / 32; ++step) {
-    const int64_t s = warp * kPlanSlotsPerWarp + step * 32 + lane;
+  for (int step = 0; step < steps; ++step) {
+    const int64_t s = (warp * steps + step) * 32 + lane;
     int e = -1;
     if (s < n_slots) {
       e = idx[s];

@@ -77,8 +77,42 @@ ROWS = [  # T, d, E, k, capacity, align, pad
     (33, 72, 40, 32, 3, 4, 9),     # k = 32
     (700, 264, 6, 2, 100, 1, 100),  # one warp per token
     (1500, 16, 3, 1, 0, 16, 0),
+    (1900, 2064, 10, 9, 0, 1, 3),   # one warp per token, several full steps and a rest; k > 8
     (9, 64, 5, 2, 0, 1, 9),        # no token has an expert
 ]
+
+
+@pytest.mark.parametrize("n,k,E,cap,align", [
+    (2049, 1, 3, 0, 1),         # just past one block
+    (20000, 4, 600, 0, 8),      # eight warps per block, several steps each, more than 512 experts
+    (33000, 8, 128, 1500, 1),   # 32 warps per block
+    (60011, 1, 4096, 3, 2),     # more experts than threads
+    (300000, 2, 2, 0, 1024)])
+def test_plan_of_many_slots(K, n, k, E, cap, align):
+    g = gen(n)
+    idx = torch.randint(-1, E, (n, k), generator=g, device="cuda", dtype=torch.int32)
+    plan = K.dispatch_plan(idx, E, cap, align)
+    flat = idx.reshape(-1).long()
+    key = torch.where(flat >= 0, flat, E)
+    order = torch.argsort(key, stable=True)
+    counts = torch.bincount(key, minlength=E + 1)[:E]
+    kept = counts.clamp(max=cap) if cap else counts
+    start = torch.zeros(E + 1, dtype=torch.int64, device="cuda")
+    start[1:] = torch.cumsum((kept + align - 1) // align * align, 0)
+    first = torch.zeros(E + 1, dtype=torch.int64, device="cuda")
+    first[1:] = torch.cumsum(counts, 0)
+    sk = key[order]
+    pos = torch.arange(n * k, device="cuda") - first[sk]
+    live = (sk < E) & (pos < (cap or n * k))
+    sr = torch.empty_like(flat)
+    sr[order] = torch.where(live, start[sk.clamp(max=E - 1)] + pos, -1)
+    assert torch.equal(plan["counts"].long(), counts) and torch.equal(plan["offsets"].long(), start)
+    assert torch.equal(plan["slot_row"].long(), sr)
+    total = int(start[E])
+    tokens = torch.full((total,), -1, dtype=torch.int64, device="cuda")
+    tokens[sr[sr >= 0]] = torch.nonzero(sr >= 0).reshape(-1) // k
+    assert torch.equal(plan["row_token"][:total].long(), tokens)
+    assert K.read_device_error("cuda") == 0
 
 
 def same_rows(rows, sr, x, w, dtype):
