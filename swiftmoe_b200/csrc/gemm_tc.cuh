@@ -68,23 +68,39 @@ struct TileCoord {
   int g, row0, rows_valid, nb;
 };
 
-// Per-launch group table, built by one thread: group g covers rows
-// [s_beg[g], s_fin[g]) -- offsets[g] .. (ends ? ends[g] : offsets[g+1]) clamped into
-// [0, rows_cap] so that no tile can touch rows outside the buffers whatever the caller
-// passed -- and its tiles are numbered from s_ts[g]; s_ts[G] is the total.
+// Per-launch group table: group g covers rows [s_beg[g], s_fin[g]) -- offsets[g] ..
+// (ends ? ends[g] : offsets[g+1]) clamped into [0, rows_cap] so that no tile can touch rows
+// outside the buffers whatever the caller passed -- and its tiles are numbered from
+// s_ts[g]; s_ts[G] is the total.  In two parts with a block barrier after each: all
+// threads read the groups' ranges and leave their tile counts in s_ts, then one warp
+// scans them.  (One thread doing both waits for every group's loads in turn: 59 against
+// 31 us for a launch over 64 groups of 78 rows.)
 template <int BM_>
-__device__ __forceinline__ void build_group_table(const int32_t* offsets, const int32_t* ends, int G, int rows_cap,
-                                                  int NB, int* s_beg, int* s_fin, int* s_ts) {
-  int acc = 0;
-  for (int g = 0; g < G; ++g) {
+__device__ __forceinline__ void load_group_table(const int32_t* offsets, const int32_t* ends, int G, int rows_cap,
+                                                 int NB, int* s_beg, int* s_fin, int* s_ts) {
+  for (int g = threadIdx.x; g < G; g += blockDim.x) {
     const int b = min(max(offsets[g], 0), rows_cap);
     const int f = min(max(ends != nullptr ? ends[g] : offsets[g + 1], b), rows_cap);
     s_beg[g] = b;
     s_fin[g] = f;
-    s_ts[g] = acc;
-    acc += ((f - b + BM_ - 1) / BM_) * NB;
+    s_ts[g] = ((f - b + BM_ - 1) / BM_) * NB;
   }
-  s_ts[G] = acc;
+}
+__device__ __forceinline__ void scan_group_table(int G, int* s_ts) {  // one whole warp
+  const int lane = threadIdx.x & 31;
+  int run = 0;
+  for (int g0 = 0; g0 < G; g0 += 32) {
+    const int n = g0 + lane < G ? s_ts[g0 + lane] : 0;
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (g0 + lane < G) s_ts[g0 + lane] = run + incl - n;
+    run += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) s_ts[G] = run;
 }
 
 // Tile L -> (group, first row, valid rows, n-block).  Inside a group the tiles are
@@ -547,10 +563,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto tempty_bar = [&](int a) { return smem_u32(bars + 2 * STAGES + 2 + a); };
   const uint32_t mma_done_bar = smem_u32(bars + 2 * STAGES + 4);
 
-  if (threadIdx.x == 0) {
-    *s_abort = 0;
-    build_group_table<BM>(offsets, ends, G, rows_cap, NB, s_beg, s_fin, s_ts);
-  }
+  if (threadIdx.x == 0) *s_abort = 0;
+  load_group_table<BM>(offsets, ends, G, rows_cap, NB, s_beg, s_fin, s_ts);
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full_bar(s), 1);
@@ -570,6 +584,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (warp == 2) scan_group_table(G, s_ts);
+  __syncthreads();
   const uint32_t tmem_base = *s_tmem;
   const int tiles = s_ts[G];
   int ks_n = 1;
@@ -738,26 +754,22 @@ __global__ void __launch_bounds__(THREADS, 1)
 // where A [M, Ktot] and B [N, Ktot] are K-major (the transposed routed rows: K runs over
 // the rows of all groups, grouped by expert).  Same pipeline as grouped_gemm_kernel
 // (TMA producer, single-thread tcgen05.mma issuer, double-buffered TMEM accumulators,
-// four epilogue warps); the tiles are 128 (M) x 256 (N) of one group, n fastest within
-// an m-tile, so a group's B rows (its K range of B) stay in L2 while the A rows stream
-// once.  Group starts must be multiples of BK (the dispatch plan's row_align 64): the
+// four epilogue warps); the tiles are 128 (M) x 256 (N) of one group.  Group starts must be multiples of BK (the dispatch plan's row_align 64): the
 // K tiles of a group then never reach into the next group, and every TMA K coordinate is
 // 16-byte aligned.  A start that is not is rounded down (wrong sums, no fault) and
 // reported in the device error word.  A group without rows gets zeros.
-// Tile L -> (group, m0, n0).  n_fast: the n-tiles of one m-tile run back to back, so a
-// group's B rows stay in L2 while A streams once (B the smaller operand); otherwise the
-// m-tiles of one n-tile do, keeping A resident instead.
-__device__ __forceinline__ void wgrad_tile(int L, int MT, int NB, bool n_fast, int& g, int& m0, int& n0) {
+// Tile L -> (group, m0, n0), in bands of `band` m-tiles, m fastest inside a band: CTAs that
+// run at the same time then share the 256-wide B tiles, the larger operand of a tile, and
+// a band's A columns and the group's B rows stay in L2.
+__device__ __forceinline__ void wgrad_tile(int L, int MT, int NB, int band, int& g, int& m0, int& n0) {
   const int per = MT * NB;
   g = L / per;
   const int local = L - g * per;
-  if (n_fast) {
-    m0 = (local / NB) * BM;
-    n0 = (local % NB) * BN;
-  } else {
-    m0 = (local % MT) * BM;
-    n0 = (local / MT) * BN;
-  }
+  const int first = local / (band * NB) * band;  // the band's first m-tile
+  const int bm = min(band, MT - first);
+  const int r = local - first * NB;
+  m0 = (first + r % bm) * BM;
+  n0 = (r / bm) * BN;
 }
 
 // fp32 tile rows through a 4 KB shared-memory stage per epilogue warp: each thread
@@ -801,15 +813,19 @@ __device__ __forceinline__ void epilogue_f32_staged(uint32_t tbase, float* __res
 // alignment -- and the last one reaches up to 63 rows past its end, into the next group.
 // Those rows must not count, and they may hold anything (Inf and NaN times zero is not
 // zero), so the MMA warp overwrites them with zeros in both operands' boxes (a K row is 128
-// contiguous bytes of every box, whatever the swizzle) before it issues the tile's MMAs,
-// and it issues only the 16-row K steps that hold rows of the group: at most 15 rows x 6
-// boxes x 128 bytes are written.
-__device__ __forceinline__ void zero_tile_rows(unsigned char* a, unsigned char* b, int valid, int upto, int lane) {
-  const int n = (upto - valid) * 8;  // 16-byte pieces per box
-  for (int i = lane; i < 6 * n; i += 32) {
-    const int box = i / n, p = i - box * n;
-    unsigned char* base = box < 2 ? a + box * kMnBox : b + (box - 2) * kMnBox;
-    *reinterpret_cast<uint4*>(base + valid * 128 + p * 16) = make_uint4(0u, 0u, 0u, 0u);
+// contiguous bytes of every box, whatever the swizzle) before lane 0 issues the tile's
+// MMAs, and it issues only the 16-row K steps that hold rows of the group: at most 15 rows
+// x 6 boxes x 128 bytes are written.  cmd: stage | valid rows << 8.  Lanes 1 to 31 wait for
+// it on the warp barrier (with all lanes following the pipeline's mbarriers instead, the
+// gradient of 8 x 14336 x 4096 weights took 2.06 ms against 1.82 at the power cap).
+__device__ __forceinline__ void zero_tile_rows(unsigned char* sA, unsigned char* sB, int cmd, int lane) {
+  const int stage = cmd & 255, valid = cmd >> 8;
+  const int n = ((valid + 15) / 16 * 16 - valid) * 8;  // 16-byte pieces per box
+#pragma unroll
+  for (int box = 0; box < 6; ++box) {
+    unsigned char* base = box < 2 ? sA + stage * A_BYTES + box * kMnBox : sB + stage * B_BYTES + (box - 2) * kMnBox;
+    for (int p = lane - 1; p < n; p += 31)
+      *reinterpret_cast<uint4*>(base + valid * 128 + p * 16) = make_uint4(0u, 0u, 0u, 0u);
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -833,7 +849,7 @@ template <typename OutT, bool MN, bool ANY = false>
 __global__ void __launch_bounds__(THREADS, 1)
     wgrad_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       OutT* __restrict__ C, const int32_t* __restrict__ koff, int G, int M, int N, uint32_t idesc,
-                      bool n_fast, int k_rows) {
+                      int band, int k_rows) {
   static_assert(!ANY || MN, "groups that start anywhere need row-major operands");
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
@@ -843,6 +859,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sB + STAGES * B_BYTES);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + NUM_BARS);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  [[maybe_unused]] volatile int* s_cmd = reinterpret_cast<volatile int*>(s_tmem + 2);  // ANY: rows to clear, -1: done
   // first and end K tile of each group; ANY: its first row and end row
   int* s_kb0 = reinterpret_cast<int*>(s_tmem + 4);
   int* s_kb1 = s_kb0 + (MAX_GROUPS + 1);
@@ -862,21 +879,17 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto tempty_bar = [&](int a) { return smem_u32(bars + 2 * STAGES + 2 + a); };
   const uint32_t mma_done_bar = smem_u32(bars + 2 * STAGES + 4);
 
-  if (threadIdx.x == 0) {
-    *s_abort = 0;
-    bool misaligned = false;
-    for (int g = 0; g < G; ++g) {
-      if constexpr (ANY) {
-        s_kb0[g] = min(max(koff[g], 0), k_rows);
-        s_kb1[g] = min(max(koff[g + 1], s_kb0[g]), k_rows);
-        continue;
-      }
+  if (threadIdx.x == 0) *s_abort = 0;
+  for (int g = threadIdx.x; g < G; g += blockDim.x) {
+    if constexpr (ANY) {
+      s_kb0[g] = min(max(koff[g], 0), k_rows);
+      s_kb1[g] = min(max(koff[g + 1], s_kb0[g]), k_rows);
+    } else {
       const int a = max(koff[g], 0), b = max(koff[g + 1], a);
-      misaligned |= (a % BK) != 0;
+      if (a % BK != 0) set_device_error(kErrBadGroupStart);
       s_kb0[g] = a / BK;                    // rounded down: a K coordinate stays aligned
       s_kb1[g] = (b + BK - 1) / BK;
     }
-    if (misaligned) set_device_error(kErrBadGroupStart);
   }
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -907,7 +920,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool ok = true;
       for (int L = blockIdx.x; L < total && ok; L += gridDim.x) {
         int g, m0, n0;
-        wgrad_tile(L, MT, NB, n_fast, g, m0, n0);
+        wgrad_tile(L, MT, NB, band, g, m0, n0);
         constexpr int STEP = ANY ? BK : 1;
         for (int kb = s_kb0[g]; kb < s_kb1[g]; kb += STEP) {
           const int k0 = ANY ? kb : kb * BK;
@@ -936,64 +949,72 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (ANY || lane == 0) {
+    if (lane == 0) {
       // ------------------------------------------------------------- MMA issuer
-      // (ANY: the whole warp follows the pipeline, to clear the rows past a group's end;
-      // lane 0 issues)
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
       bool ok = true;
-      auto wait = [&](uint32_t bar, uint32_t parity) {
-        const bool got = mbar_wait(bar, parity, s_abort);
-        return ANY ? __all_sync(0xffffffffu, got) != 0 : got;
-      };
       for (int L = blockIdx.x; L < total && ok; L += gridDim.x) {
         int g, m0, n0;
-        wgrad_tile(L, MT, NB, n_fast, g, m0, n0);
+        wgrad_tile(L, MT, NB, band, g, m0, n0);
         const int kb0 = s_kb0[g], kb1 = s_kb1[g];
         if (kb1 <= kb0) continue;           // no rows: the epilogue writes zeros
-        if (!wait(tempty_bar(acc), acc_phase ^ 1)) break;
+        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1, s_abort)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
         constexpr int STEP = ANY ? BK : 1;
         for (int kb = kb0; kb < kb1; kb += STEP) {
-          if (!wait(full_bar(stage), phase)) { ok = false; break; }
+          if (!mbar_wait(full_bar(stage), phase, s_abort)) { ok = false; break; }
           int steps = BK / 16;
           if constexpr (ANY) {
-            const int valid = min(BK, kb1 - kb);
-            steps = (valid + 15) / 16;
-            if (valid < 16 * steps) zero_tile_rows(sA + stage * A_BYTES, sB + stage * B_BYTES, valid, 16 * steps, lane);
-            __syncwarp();
+            const int valid = kb1 - kb;
+            if (valid < BK) {               // the group's last rows
+              steps = (valid + 15) / 16;
+              if (valid < 16 * steps) {     // wake the other lanes, wait for them
+                *s_cmd = stage | valid << 8;
+                __syncwarp();
+                __syncwarp();
+              }
+            }
           }
           tc_fence_after();
-          if (lane == 0) {
 #pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk) {
-              if (ANY && kk >= steps) break;
-              uint64_t a_desc, b_desc;
-              if constexpr (MN) {   // K step of 16 rows = two 1 KB atoms along K
-                a_desc = umma_desc_mn_sw128(smem_u32(sA + stage * A_BYTES) + kk * 2048, kMnBox, 1024);
-                b_desc = umma_desc_mn_sw128(smem_u32(sB + stage * B_BYTES) + kk * 2048, kMnBox, 1024);
-              } else {              // K step of 16 elements = 32 bytes inside the 128-byte rows
-                a_desc = umma_desc_sw128(smem_u32(sA + stage * A_BYTES)) + 2 * kk;
-                b_desc = umma_desc_sw128(smem_u32(sB + stage * B_BYTES)) + 2 * kk;
-              }
-              umma_f16(d_tmem, a_desc, b_desc, idesc, (kb > kb0 || kk != 0) ? 1u : 0u);
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            if (ANY && kk >= steps) break;
+            uint64_t a_desc, b_desc;
+            if constexpr (MN) {   // K step of 16 rows = two 1 KB atoms along K
+              a_desc = umma_desc_mn_sw128(smem_u32(sA + stage * A_BYTES) + kk * 2048, kMnBox, 1024);
+              b_desc = umma_desc_mn_sw128(smem_u32(sB + stage * B_BYTES) + kk * 2048, kMnBox, 1024);
+            } else {              // K step of 16 elements = 32 bytes inside the 128-byte rows
+              a_desc = umma_desc_sw128(smem_u32(sA + stage * A_BYTES)) + 2 * kk;
+              b_desc = umma_desc_sw128(smem_u32(sB + stage * B_BYTES)) + 2 * kk;
             }
-            umma_commit(empty_bar(stage));
+            umma_f16(d_tmem, a_desc, b_desc, idesc, (kb > kb0 || kk != 0) ? 1u : 0u);
           }
+          umma_commit(empty_bar(stage));
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
-        if (lane == 0) umma_commit(tfull_bar(acc));
+        umma_commit(tfull_bar(acc));
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
-      if (lane == 0) {
-        umma_commit(mma_done_bar);
-        mbar_wait_drain(mma_done_bar, 0);
+      if constexpr (ANY) {                  // the other lanes may leave
+        *s_cmd = -1;
+        __syncwarp();
+      }
+      umma_commit(mma_done_bar);
+      mbar_wait_drain(mma_done_bar, 0);
+    } else if constexpr (ANY) {
+      // asleep on the warp barrier until lane 0 has rows to clear
+      while (true) {
+        __syncwarp();
+        const int cmd = *s_cmd;
+        if (cmd < 0) break;
+        zero_tile_rows(sA, sB, cmd, lane);
+        __syncwarp();
       }
     }
   } else {
@@ -1004,7 +1025,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t acc_phase = 0;
     for (int L = blockIdx.x; L < total; L += gridDim.x) {
       int g, m0, n0;
-      wgrad_tile(L, MT, NB, n_fast, g, m0, n0);
+      wgrad_tile(L, MT, NB, band, g, m0, n0);
       const uint32_t tq = tmem_base + ((uint32_t)(q * 32) << 16);
       if constexpr (sizeof(OutT) == 2) {    // one rounding to 16 bits, rows staged as in EPI_ROWS
         const int row = m0 + q * 32 + lane;
@@ -1116,10 +1137,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   auto tempty_bar = [&](int a) { return smem_u32(bars + 2 * STAGES + 2 + a); };
   const uint32_t mma_done_bar = smem_u32(bars + 2 * STAGES + 4);
 
-  if (threadIdx.x == 0) {
-    *s_abort = 0;
-    build_group_table<BM>(offsets, ends, G, rows_cap, NB, s_beg, s_fin, s_ts);
-  }
+  if (threadIdx.x == 0) *s_abort = 0;
+  load_group_table<BM>(offsets, ends, G, rows_cap, NB, s_beg, s_fin, s_ts);
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full_bar(s), 1);
@@ -1140,6 +1159,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   __syncthreads();
   cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA arrive
   tc_fence_after();
+  if (warp == 2) scan_group_table(G, s_ts);
+  __syncthreads();
   const uint32_t tmem_base = *s_tmem;
   const int total = s_ts[G];
 

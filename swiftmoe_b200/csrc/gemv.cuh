@@ -82,11 +82,16 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_gemv_kernel(const T* __res
     s_fin[g] = min(max(ends != nullptr ? ends[g] : offsets[g + 1], b), min(rows_cap, b + MAX_ROWS));
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 32) {  // one warp compacts them, 32 groups at a time
     int n = 0;
-    for (int g = 0; g < G; ++g)
-      if (s_fin[g] > s_beg[g]) s_act[n++] = g;
-    s_nact = n;
+    for (int g0 = 0; g0 < G; g0 += 32) {
+      const int g = g0 + (int)threadIdx.x;
+      const bool has = g < G && s_fin[g] > s_beg[g];
+      const unsigned m = __ballot_sync(0xffffffffu, has);
+      if (has) s_act[n + __popc(m & ((1u << threadIdx.x) - 1u))] = g;
+      n += __popc(m);
+    }
+    if (threadIdx.x == 0) s_nact = n;
   }
   __syncthreads();
   if constexpr (EPI == EPI_LINEAR) {

@@ -85,6 +85,6 @@ def test_workspace_sizes(lib):
     assert lib.smoe_grouped_linear_workspace_size(2, 4096, L.SMOE_W_KN) > 0
     assert lib.smoe_grouped_linear_workspace_size(64, 4096, L.SMOE_W_NK) > 0
     assert lib.smoe_grouped_linear_workspace_size(16384, 4096, L.SMOE_W_NK) == 0
-    # bias partials: at most 64 slices of at least 64 rows, plus one row per group
-    assert lib.smoe_linear_act_bwd_workspace_size(64, 8, 4) == (1 + 4) * 8 * 4
-    assert lib.smoe_linear_act_bwd_workspace_size(1 << 20, 8, 4) == (64 + 4) * 8 * 4
+    # bias partials: a row per slice (16 to 512 rows) and one per group
+    assert lib.smoe_linear_act_bwd_workspace_size(64, 8, 4) == (4 + 4) * 8 * 4
+    assert lib.smoe_linear_act_bwd_workspace_size(1 << 20, 8, 4) == ((1 << 20) // 512 + 4) * 8 * 4
