@@ -233,7 +233,7 @@ SMOE_API int smoe_grouped_gemm_rows(const void* A, const void* B, const void* B3
  * split K over otherwise idle SMs through the workspace (its size may be 0).
  * Replaces: nn.Linear experts with a bias around models/baseline_moe.py:151-162 (the
  * reference's own are bias-free and linear).                                           */
-SMOE_API size_t smoe_grouped_linear_workspace_size(int64_t rows_cap, int N, int w_layout);
+SMOE_API size_t smoe_grouped_linear_workspace_size(int64_t rows_cap, int N, int K, int G, int w_layout);
 SMOE_API int smoe_grouped_linear(const void* A, const void* W, int w_layout, const void* bias, int bias_dtype, int act,
                                  const void* residual, void* preact, int fill, void* C, int dtype,
                                  const int32_t* offsets, int G, int64_t rows_cap, int N, int K, void* workspace,
@@ -248,9 +248,11 @@ SMOE_API int smoe_linear_act_bwd(const void* dout, const void* preact, int act, 
                                  size_t workspace_bytes, smoe_stream_t stream);
 /* Weight gradient dW[g] = dz_g^T A_g, [G, N, K] in dtype or fp32 (out_dtype), dz
  * [rows_cap, N], A [rows_cap, K].  Groups may start at any row; a group without rows gets
- * zeros.  The input gradient is smoe_grouped_linear(dz, W, SMOE_W_KN).                  */
+ * zeros.  Few tiles are split along the rows through the workspace (its size may be 0).  The input gradient is smoe_grouped_linear(dz, W, SMOE_W_KN).                  */
+SMOE_API size_t smoe_linear_wgrad_workspace_size(int64_t rows_cap, int G, int N, int K);
 SMOE_API int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const int32_t* offsets, int G,
-                               int64_t rows_cap, int N, int K, void* dW, int out_dtype, smoe_stream_t stream);
+                               int64_t rows_cap, int N, int K, void* dW, int out_dtype, void* workspace,
+                               size_t workspace_bytes, smoe_stream_t stream);
 
 /* out[r, :] = [lo(w[r, :]) | hi(w[r, :]) | hi(w[r, :])] for `rows` fp32 rows of K (K % 4
  * == 0, 16-byte aligned): hi = the tf32 rounding (to nearest, ties away from zero), lo =

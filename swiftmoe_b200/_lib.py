@@ -75,12 +75,13 @@ SIGNATURES = {
     "smoe_sort_tokens": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp,
                                 _vp, _sz, _vp]),
     "smoe_unsort_rows": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp]),
-    "smoe_grouped_linear_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "smoe_grouped_linear_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32]),
     "smoe_grouped_linear": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _i32, _i64, _i32,
                                    _i32, _vp, _sz, _vp]),
     "smoe_linear_act_bwd_workspace_size": (_sz, [_i64, _i32, _i32]),
     "smoe_linear_act_bwd": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _i64, _i32, _vp, _sz, _vp]),
-    "smoe_linear_wgrad": (_i32, [_vp, _vp, _i32, _vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp]),
+    "smoe_linear_wgrad_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
+    "smoe_linear_wgrad": (_i32, [_vp, _vp, _i32, _vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp, _sz, _vp]),
     "smoe_grouped_gemm": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _vp]),
     "smoe_grouped_gemm_rows": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _vp]),
     "smoe_transpose_batched": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp]),

@@ -21,6 +21,7 @@
 #include "gemm_simt.cuh"
 #include "gemv.cuh"
 #include "gemm_tc.cuh"
+#include "gemm_linear.cuh"
 #include "routed_rows.cuh"
 #include "router.cuh"
 
@@ -317,19 +318,18 @@ void* tf32_scratch(cudaStream_t st, size_t bytes) {
 
 // forced: a split-K scratch of the caller's with at least min_split slices per tile;
 // otherwise the stream's own (the kernel then splits only launches with few tiles).
-template <int EPI, typename OutT, int ES = 2, bool BMN = false>
+template <int EPI, typename OutT, int ES = 2>
 int launch_tc(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mb3, void* C, int64_t ldc,
               const uint64_t* row_ptrs, const int32_t* offsets, const int32_t* ends, int G, int64_t rows_cap, int N, int K, uint32_t idesc,
-              cudaStream_t st, const SplitScratch* forced = nullptr, int min_split = 1,
-              const LinearEpi& lin = LinearEpi()) {
+              cudaStream_t st, const SplitScratch* forced = nullptr, int min_split = 1) {
   static SmemGrant done;
-  auto kern = tc::grouped_gemm_kernel<EPI, OutT, ES, BMN>;
+  auto kern = tc::grouped_gemm_kernel<EPI, OutT, ES>;
   constexpr int smem = EPI == tc::EPI_ROWS ? tc::SMEM_BYTES_ROWS : tc::SMEM_BYTES;
   SMOE_CK(ensure_smem(kern, smem, &done));
   const SplitScratch sc = forced ? *forced : split_scratch(st);
   SMOE_CK(launch_k(kern, device_sms(), tc::THREADS, smem, st, ma, mb, mb3, reinterpret_cast<OutT*>(C), ldc, row_ptrs, offsets, ends, G, N,
                                                          K, (int)rows_cap, raster_band(EPI), idesc, sc.ws, sc.cnt, sc.units,
-                                                         forced ? min_split : 1, lin));
+                                                         forced ? min_split : 1));
   SMOE_CK(cudaGetLastError());
   return SMOE_OK;
 }
@@ -352,15 +352,15 @@ int launch_tc_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorM
 // rows, at the power cap: n fastest 1.83 ms, bands of 8 / 16 / 32 m-tiles 1.52 / 1.52 / 1.50 ms.
 constexpr int kWgradBand = 32;
 
-template <bool MN, typename OutT = float, bool ANY = false>
-int launch_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, OutT* C, const int32_t* koff, int G, int M, int N,
-                 uint32_t idesc, cudaStream_t st, int k_rows = 0) {
+template <bool MN>
+int launch_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, float* C, const int32_t* koff, int G, int M, int N,
+                 uint32_t idesc, cudaStream_t st) {
   static SmemGrant done;
-  auto kern = tc::wgrad_gemm_kernel<OutT, MN, ANY>;
+  auto kern = tc::wgrad_gemm_kernel<float, MN>;
   SMOE_CK(ensure_smem(kern, tc::SMEM_BYTES_ROWS, &done));
   const int64_t tiles = (int64_t)G * cdiv(M, tc::BM) * cdiv(N, tc::BN);
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sms()));
-  kern<<<grid, tc::THREADS, tc::SMEM_BYTES_ROWS, st>>>(ma, mb, C, koff, G, M, N, idesc, kWgradBand, k_rows);
+  kern<<<grid, tc::THREADS, tc::SMEM_BYTES_ROWS, st>>>(ma, mb, C, koff, G, M, N, idesc, kWgradBand);
   SMOE_CK(cudaGetLastError());
   return SMOE_OK;
 }
@@ -610,40 +610,87 @@ bool make_map_3d_mn(CUtensorMap* m, const void* base, CUtensorMapDataType dt, in
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Split-K scratch of a linear layer: the caller's workspace, so that graphs captured on
-// one stream and replayed on several never share it.  Wanted where the rows, were they all
-// of one group, would make at most half as many tiles as SMs (the kernel's own condition,
-// on the device, is the same on the groups' real tiles).
-constexpr size_t kSplitSlot = (size_t)tc::BM * tc::BN * sizeof(float);
-size_t linear_workspace(int64_t rows_cap, int N) {
-  const int units = device_sms();
-  if (rows_cap < 1 || 2 * cdiv(rows_cap, tc::BM) * cdiv(N, tc::BN) > units) return 0;
-  return (size_t)units * (kSplitSlot + sizeof(int));
+// Partial tiles of a split launch (lin::split_units): rows and number of the slots in the
+// caller's workspace -- the caller's, so that graphs captured on one stream and replayed on
+// several never share it -- at most 64 MB.  No slots where neither evenly filled groups nor
+// all rows in one group would make a split worth it, the kernel then decides on the groups'
+// real tiles.
+constexpr int64_t kSplitBytes = 64 << 20;
+
+struct SplitPlan {
+  int rows = 0, slots = 0;
+  size_t bytes() const { return (size_t)slots * rows * lin::BN * sizeof(float); }
+};
+
+SplitPlan linear_split_plan(int64_t rows_cap, int N, int K, int G) {
+  SplitPlan p;
+  if (rows_cap < 1) return p;
+  p.rows = (int)std::min<int64_t>(lin::BM, align_up((size_t)rows_cap, 8));
+  const int64_t slots = std::min<int64_t>(kSplitBytes / ((int64_t)p.rows * lin::BN * 4), (int64_t)device_sms() * lin::MAX_SPLIT);
+  const int64_t nb = cdiv(N, lin::BN), groups = std::min<int64_t>(G, rows_cap);
+  const int64_t even = groups * cdiv(cdiv(rows_cap, groups), lin::BM) * nb, one = cdiv(rows_cap, lin::BM) * nb;
+  const int kb = (int)cdiv(K, lin::BK);
+  for (int64_t tiles : {even, one})
+    if (lin::split_units(tiles, kb, p.rows, device_sms(), slots) > 1) p.slots = (int)slots;
+  return p;
 }
+
+// The raster band of a product, as raster_band(): short rows of A (up to 8 KB) in bands of a
+// whole expert, longer ones half as high.
+int linear_band(int K) { return K <= 4096 ? 32 : tc::GM_DEFAULT; }
 
 template <typename T, bool BMN>
 int linear_gemm_t(const void* A, const void* B, void* C, const int32_t* offsets, int G, int64_t rows_cap, int N, int K,
-                  const LinearEpi& lin, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+                  const LinearEpi& epi, void* workspace, size_t workspace_bytes, cudaStream_t st) {
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
   if (!BMN && rows_cap <= gemv::DISPATCH_ROWS)  // decode: the weights of the groups with rows, streamed once
     return launch_gemv_t<gemv::EPI_LINEAR, T, T>(A, B, nullptr, C, nullptr, offsets, nullptr, G, rows_cap, N, K, st,
-                                                 nullptr, (int)rows_cap, lin);
+                                                 nullptr, (int)rows_cap, epi);
+  const SplitPlan sp = linear_split_plan(rows_cap, N, K, G);
+  if (sp.slots > 0 && (!workspace || workspace_bytes < sp.bytes())) return SMOE_ERR_WORKSPACE;
+  float* ws = sp.slots > 0 ? static_cast<float*>(workspace) : nullptr;
   const CUtensorMapDataType dt = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap ma, mb;
   if (!make_map_2d(&ma, A, dt, rows_cap, K)) return SMOE_ERR_CUDA;
   if (BMN ? !make_map_3d_mn(&mb, B, dt, G, K, N) : !make_map_3d(&mb, B, dt, G, N, K)) return SMOE_ERR_CUDA;
-  const uint32_t idesc = umma_idesc_f16(bf ? 1u : 0u, tc::BM, tc::BN) | (BMN ? 1u << 16 : 0u);  // transpose-B bit
-  SplitScratch sc;  // without units: no split
-  const size_t need = linear_workspace(rows_cap, N);
-  if (need > 0) {
-    if (!workspace || workspace_bytes < need) return SMOE_ERR_WORKSPACE;
-    sc.units = device_sms();
-    sc.ws = static_cast<float*>(workspace);
-    sc.cnt = reinterpret_cast<int*>(static_cast<char*>(workspace) + (size_t)sc.units * kSplitSlot);
-    SMOE_CK(cudaMemsetAsync(sc.cnt, 0, (size_t)sc.units * sizeof(int), st));
+  const uint32_t idesc = umma_idesc_f16(bf ? 1u : 0u, lin::BM, lin::BN) | (BMN ? 1u << 16 : 0u);  // transpose-B bit
+  static SmemGrant done;
+  auto kern = lin::linear_gemm_kernel<T, BMN>;
+  SMOE_CK(ensure_smem(kern, lin::SMEM_BYTES, &done));
+  const int grid = device_sms(), band = linear_band(K);
+  SMOE_CK(launch_k(kern, grid, lin::THREADS, lin::SMEM_BYTES, st, ma, mb, (T*)C, offsets, G, N, K, (int)rows_cap, band,
+                   idesc, epi, ws, sp.slots, sp.rows));
+  if (ws) {
+    const PdlScope pdl(true);
+    SMOE_CK(launch_k(lin::linear_sum_kernel<T>, grid * 4, 256, 0, st, (T*)C, offsets, G, N, K, (int)rows_cap, band, epi,
+                     ws, sp.slots, sp.rows, grid));
   }
-  return launch_tc<tc::EPI_LINEAR, T, 2, BMN>(ma, mb, mb, C, N, nullptr, offsets, nullptr, G, rows_cap, N, K, idesc, st,
-                                              &sc, 1, lin);
+  return SMOE_OK;
+}
+
+// K slices of a weight gradient's tiles, for evenly filled groups.
+int wgrad_slices(int64_t rows_cap, int G, int N, int K) {
+  const int64_t tiles = (int64_t)G * cdiv(N, lin::BM) * cdiv(K, lin::BN);
+  const int kb = (int)cdiv(cdiv(rows_cap, G), lin::BK);
+  return lin::split_units(tiles, kb, lin::BM, device_sms(), kSplitBytes / (lin::BM * lin::BN * 4));
+}
+
+template <typename OutT>
+int launch_linear_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, void* C, const int32_t* offsets, int G, int M,
+                        int N, int rows, uint32_t idesc, float* ws, int ks, cudaStream_t st) {
+  static SmemGrant done;
+  auto kern = lin::linear_wgrad_kernel<OutT>;
+  SMOE_CK(ensure_smem(kern, lin::SMEM_BYTES, &done));
+  const int64_t units = (int64_t)G * cdiv(M, lin::BM) * cdiv(N, lin::BN) * ks;
+  const int grid = (int)std::min<int64_t>(units, device_sms());
+  SMOE_CK(launch_k(kern, grid, lin::THREADS, lin::SMEM_BYTES, st, ma, mb, (OutT*)C, offsets, G, M, N, rows, kWgradBand,
+                   idesc, ws, ks));
+  if (ks > 1) {
+    const PdlScope pdl(true);
+    SMOE_CK(launch_k(lin::linear_wgrad_sum_kernel<OutT>, device_sms() * 4, 256, 0, st, (OutT*)C, offsets, G, M, N, rows,
+                     kWgradBand, ws, ks));
+  }
+  return SMOE_OK;
 }
 
 // Rows of one block (and of one partial sum of the bias gradient): a multiple of its eight
@@ -1144,9 +1191,9 @@ int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const fl
 #undef SMOE_ROWS_DISPATCH
 #undef SMOE_ROWS_CASE
 
-size_t smoe_grouped_linear_workspace_size(int64_t rows_cap, int N, int w_layout) {
-  if (rows_cap < 1 || N < 1 || (w_layout == SMOE_W_NK && rows_cap <= gemv::DISPATCH_ROWS)) return 0;
-  return linear_workspace(rows_cap, N);
+size_t smoe_grouped_linear_workspace_size(int64_t rows_cap, int N, int K, int G, int w_layout) {
+  if (rows_cap < 1 || N < 1 || K < 1 || G < 1 || (w_layout == SMOE_W_NK && rows_cap <= gemv::DISPATCH_ROWS)) return 0;
+  return linear_split_plan(rows_cap, N, K, G).bytes();
 }
 
 int smoe_grouped_linear(const void* A, const void* W, int w_layout, const void* bias, int bias_dtype, int act,
@@ -1225,8 +1272,14 @@ int smoe_linear_act_bwd(const void* dout, const void* preact, int act, void* dz,
   return SMOE_OK;
 }
 
+size_t smoe_linear_wgrad_workspace_size(int64_t rows_cap, int G, int N, int K) {
+  if (rows_cap < 1 || G < 1 || N < 1 || K < 1) return 0;
+  const int ks = wgrad_slices(rows_cap, G, N, K);
+  return ks > 1 ? (size_t)G * cdiv(N, lin::BM) * cdiv(K, lin::BN) * ks * lin::BM * lin::BN * sizeof(float) : 0;
+}
+
 int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const int32_t* offsets, int G, int64_t rows_cap, int N,
-                      int K, void* dW, int out_dtype, smoe_stream_t stream) {
+                      int K, void* dW, int out_dtype, void* workspace, size_t workspace_bytes, smoe_stream_t stream) {
   if (G < 1 || N < 1 || K < 1 || rows_cap < 0 || !offsets || !dW) return SMOE_ERR_INVALID;
   if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_UNSUPPORTED;
   if (out_dtype != dtype && out_dtype != SMOE_F32) return SMOE_ERR_UNSUPPORTED;
@@ -1237,18 +1290,21 @@ int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const int32_t* o
     return SMOE_OK;
   }
   if (!dz || !A) return SMOE_ERR_INVALID;
-  if (!aligned16(dz) || !aligned16(A) || !aligned16(dW)) return SMOE_ERR_UNSUPPORTED;
-  if ((int64_t)G * cdiv(N, tc::BM) * cdiv(K, tc::BN) > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (!aligned16(dz) || !aligned16(A) || !aligned16(dW) || !aligned16(workspace)) return SMOE_ERR_UNSUPPORTED;
+  if ((int64_t)G * cdiv(N, tc::BM) * cdiv(K, tc::BN) * lin::MAX_SPLIT > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
   const bool bf = dtype == SMOE_BF16;
   const CUtensorMapDataType dt = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap ma, mb;
+  const int ks = wgrad_slices(rows_cap, G, N, K);
+  float* ws = static_cast<float*>(workspace);
+  if (ks > 1 && (!ws || workspace_bytes < smoe_linear_wgrad_workspace_size(rows_cap, G, N, K))) return SMOE_ERR_WORKSPACE;
   if (!make_map_2d_box(&ma, dz, dt, rows_cap, N, N, tc::BK)) return SMOE_ERR_CUDA;
   if (!make_map_2d_box(&mb, A, dt, rows_cap, K, K, tc::BK)) return SMOE_ERR_CUDA;
   const uint32_t idesc = umma_idesc_f16_mn(bf ? 1u : 0u, tc::BM, tc::BN);
   const int kr = (int)rows_cap;
-  if (out_dtype == SMOE_F32) return launch_wgrad<true, float, true>(ma, mb, (float*)dW, offsets, G, N, K, idesc, st, kr);
-  return bf ? launch_wgrad<true, __nv_bfloat16, true>(ma, mb, (__nv_bfloat16*)dW, offsets, G, N, K, idesc, st, kr)
-            : launch_wgrad<true, __half, true>(ma, mb, (__half*)dW, offsets, G, N, K, idesc, st, kr);
+  if (out_dtype == SMOE_F32) return launch_linear_wgrad<float>(ma, mb, dW, offsets, G, N, K, kr, idesc, ws, ks, st);
+  return bf ? launch_linear_wgrad<__nv_bfloat16>(ma, mb, dW, offsets, G, N, K, kr, idesc, ws, ks, st)
+            : launch_linear_wgrad<__half>(ma, mb, dW, offsets, G, N, K, kr, idesc, ws, ks, st);
 }
 
 int smoe_grouped_gemm(const void* A, const void* B, const void* B3, void* C, int dtype, int out_dtype, int epilogue,

@@ -17,7 +17,6 @@
 // Every mbarrier wait is bounded (see mbar_wait); on a timeout the kernel records the
 // error, drains its in-flight copies and MMAs and frees its TMEM before returning.
 #pragma once
-#include "activation.cuh"
 #include "common.cuh"
 
 namespace smoe {
@@ -43,9 +42,6 @@ constexpr int EPI_ROWS = 2;
 // side by side, C[r, n] = A B1_g^T and C[r, N + n] = A B3_g^T (C is [rows_cap, 2N]);
 // the backward pass recomputes them instead of keeping them from the forward.
 constexpr int EPI_GATEUP = SMOE_EPI_GATEUP;
-// Internal epilogue kind of the grouped linear layers (smoe_grouped_linear): bias,
-// activation and residual in the epilogue, see LinearEpi.
-constexpr int EPI_LINEAR = 4;
 template <int EPI> struct EpiTraits {
   static constexpr bool kPair = EPI == SMOE_EPI_SWIGLU || EPI == EPI_GATEUP;  // [gate | up] tiles
 };
@@ -274,67 +270,6 @@ __device__ __forceinline__ void epilogue_tile(uint32_t tbase, OutT* crow, bool r
   }
 }
 
-// EPI_LINEAR: this thread's accumulator row plus bias, through the activation, plus the
-// residual row; 32 columns at a time.  The bias pieces are the same for every lane (one
-// broadcast load each); the residual's 64 bytes are requested before the activation.
-template <typename T>
-__device__ __forceinline__ void epilogue_linear(uint32_t tbase, int g, int row, bool row_ok, int col0, int N,
-                                                T* __restrict__ C, const LinearEpi& lin) {
-  const int64_t at = (int64_t)row * N;
-#pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
-    const int col = col0 + c * 32;
-    if (col >= N) break;  // warp-uniform
-    uint32_t v[32];
-    tmem_ld32(tbase + c * 32, v);
-    uint4 res[4];
-    const bool add = lin.residual != nullptr && row_ok;
-    if (add) {
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(lin.residual) + at + col);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) res[j] = col + 8 * j < N ? src[j] : make_uint4(0u, 0u, 0u, 0u);
-    }
-    tmem_ld_wait();
-    float f[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (col + 8 * j < N) {
-        float b[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = f[8 * j + i];
-        add_bias<T>(lin, (int64_t)g * N + col + 8 * j, b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[8 * j + i] = b[i];
-      }
-    if (lin.preact != nullptr && row_ok) Store16<T>::cols32(static_cast<T*>(lin.preact) + at, col, N, f);
-    apply_act(lin.act, f);
-    if (add)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const T* e = reinterpret_cast<const T*>(&res[j]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[8 * j + i] += Num<T>::to_f(e[i]);
-      }
-    if (row_ok) Store16<T>::cols32(C + at, col, N, f);
-  }
-}
-
-// EPI_LINEAR with lin.fill: the rows of no group, [0, first) and [last, rows_cap), become
-// the residual (zeros without one).  Threads et of nt of block b of nb.
-template <typename T>
-__device__ __forceinline__ void fill_other_rows(const LinearEpi& lin, T* __restrict__ C, int first, int last,
-                                                int rows_cap, int N, int b, int nb, int et, int nt) {
-  const int64_t pieces = (int64_t)N / 8, head = (int64_t)first * pieces;
-  const int64_t total = head + (int64_t)(rows_cap - last) * pieces;
-  for (int64_t i = (int64_t)b * nt + et; i < total; i += (int64_t)nb * nt) {
-    const int64_t p = i < head ? i : (int64_t)last * pieces + (i - head);
-    reinterpret_cast<uint4*>(C)[p] =
-        lin.residual != nullptr ? static_cast<const uint4*>(lin.residual)[p] : make_uint4(0u, 0u, 0u, 0u);
-  }
-}
-
 // -------------------------------------------------------------- fp32 on tf32 tensor cores
 // An fp32 product a*b on tf32 tensor cores to about fp32 accuracy ("3xTF32"): with
 // hi(v) = v rounded to tf32 (10 explicit mantissa bits, to nearest, ties away from zero)
@@ -429,7 +364,7 @@ template <> __device__ __forceinline__ void store4<float>(float* p, float a, flo
 // serialise them.
 template <int EPI, typename OutT>
 __device__ __forceinline__ void split_fixup(const float* tile_ws, int ks_n, const TileCoord& t, OutT* C, int64_t ldc,
-                                            const uint64_t* row_ptrs, int N, int et, const LinearEpi& lin) {
+                                            const uint64_t* row_ptrs, int N, int et) {
   constexpr bool kPair = EpiTraits<EPI>::kPair;
   constexpr int U = kPair ? 4 : 8, QB = 4;
   const int col0 = kPair ? t.nb * 128 : t.nb * BN;
@@ -491,27 +426,12 @@ __device__ __forceinline__ void split_fixup(const float* tile_ws, int ks_n, cons
       } else if constexpr (EPI == EPI_GATEUP) {
         store4<OutT>(dst + col0 + c, x.x, x.y, x.z, x.w);
         store4<OutT>(dst + N + col0 + c, y.x, y.y, y.z, y.w);
-      } else if constexpr (EPI == EPI_LINEAR) {
-        const int64_t at = (int64_t)(t.row0 + row) * N + col0 + c;
-        float f[4] = {x.x, x.y, x.z, x.w};
-        add_bias<OutT>(lin, (int64_t)t.g * N + col0 + c, f);
-        if (lin.preact != nullptr) store4<OutT>(static_cast<OutT*>(lin.preact) + at, f[0], f[1], f[2], f[3]);
-        apply_act(lin.act, f);
-        if (lin.residual != nullptr) {
-          const uint2 rv = *reinterpret_cast<const uint2*>(static_cast<const OutT*>(lin.residual) + at);
-          const OutT* e = reinterpret_cast<const OutT*>(&rv);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) f[q] += Num<OutT>::to_f(e[q]);
-        }
-        store4<OutT>(dst + col0 + c, f[0], f[1], f[2], f[3]);
       } else {
         store4<OutT>(dst + col0 + c, x.x, x.y, x.z, x.w);
       }
     }
   }
 }
-
-constexpr uint32_t kMnBox = 64 * BK * 2;  // one 64 x 64 MN-major box: 8 KB
 
 // EPI: SMOE_EPI_STORE or SMOE_EPI_SWIGLU.  OutT: float, __nv_bfloat16 or __half.
 // split_ws / split_cnt: split-K scratch of split_units fp32 [BM, BN] slots and as many
@@ -522,17 +442,13 @@ constexpr uint32_t kMnBox = 64 * BK * 2;  // one 64 x 64 MN-major box: 8 KB
 // ES: operand element size -- 2 for bf16/fp16 (kind::f16, 64 elements per 128-byte
 // swizzle row), 4 for tf32 (fp32 operands, kind::tf32, 32 elements per row); either way a
 // k-block is one 128-byte row per operand row and 4 MMAs of 32 bytes of K.
-// BMN: the product with B itself instead of its transpose, C = A B_g for B [G, K, N] (the
-// input gradient of a linear layer, whose weights are stored [outputs, inputs]): a stage
-// holds four boxes of 64 columns x 64 rows of K of B, read as an MN-major operand, so no
-// transposed copy of the weights is made.
-template <int EPI, typename OutT, int ES = 2, bool BMN = false>
+template <int EPI, typename OutT, int ES = 2>
 __global__ void __launch_bounds__(THREADS, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmB3, OutT* __restrict__ C, int64_t ldc, const uint64_t* __restrict__ row_ptrs,
                         const int32_t* __restrict__ offsets, const int32_t* __restrict__ ends, int G, int N,
                         int K, int rows_cap, int gm, uint32_t idesc, float* __restrict__ split_ws,
-                        int* __restrict__ split_cnt, int split_units, int min_split, const LinearEpi lin) {
+                        int* __restrict__ split_cnt, int split_units, int min_split) {
   pdl_wait();
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
@@ -614,14 +530,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint32_t a_dst = smem_u32(sA + stage * A_BYTES);
           const uint32_t b_dst = smem_u32(sB + stage * B_BYTES);
           tma_load_2d(a_dst, &tmA, fb, kb * BKE, t.row0);
-          if constexpr (BMN) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) tma_load_3d(b_dst + i * kMnBox, &tmB, fb, n0 + 64 * i, kb * BKE, t.g);
-          } else {
-            tma_load_3d(b_dst, &tmB, fb, kb * BKE, n0, t.g);
-            if (kPair) tma_load_3d(b_dst + B_BYTES / 2, &tmB3, fb, kb * BKE, n0, t.g);
-            else tma_load_3d(b_dst + B_BYTES / 2, &tmB, fb, kb * BKE, n0 + 128, t.g);
-          }
+          tma_load_3d(b_dst, &tmB, fb, kb * BKE, n0, t.g);
+          if (kPair) tma_load_3d(b_dst + B_BYTES / 2, &tmB3, fb, kb * BKE, n0, t.g);
+          else tma_load_3d(b_dst + B_BYTES / 2, &tmB, fb, kb * BKE, n0 + 128, t.g);
           ++issued;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
@@ -653,11 +564,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint64_t b_desc = umma_desc_sw128(smem_u32(sB + stage * B_BYTES));
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {  // 32 bytes of K each: 16 f16 or 8 tf32 elements
-            if constexpr (BMN)  // K step of 16 rows = two 1 KB atoms of the MN-major B tile
-              umma_f16(d_tmem, a_desc + 2 * kk,
-                       umma_desc_mn_sw128(smem_u32(sB + stage * B_BYTES) + kk * 2048, kMnBox, 1024), idesc,
-                       (kb != kb_lo || kk != 0) ? 1u : 0u);
-            else if constexpr (ES == 4)
+            if constexpr (ES == 4)
               umma_tf32(d_tmem, a_desc + 2 * kk, b_desc + 2 * kk, idesc, (kb != kb_lo || kk != 0) ? 1u : 0u);
             else
               umma_f16(d_tmem, a_desc + 2 * kk, b_desc + 2 * kk, idesc, (kb != kb_lo || kk != 0) ? 1u : 0u);
@@ -679,10 +586,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int r = q * 32 + lane;
     int acc = 0;
     uint32_t acc_phase = 0;
-    if constexpr (EPI == EPI_LINEAR)  // while the first tile is computed
-      if (lin.fill)
-        fill_other_rows<OutT>(lin, C, s_beg[0], s_fin[G - 1], rows_cap, N, blockIdx.x, gridDim.x,
-                              (int)threadIdx.x - 64, 128);
     for (int L = blockIdx.x; L < total; L += gridDim.x) {
       const int tile = L / ks_n;
       const TileCoord t = decode_tile_t<BM>(tile, s_ts, s_beg, s_fin, G, NB, gm);
@@ -717,7 +620,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (last) {
           __threadfence();
           split_fixup<EPI, OutT>(split_ws + (int64_t)tile * ks_n * BM * BN, ks_n, t, C, ldc, row_ptrs, N,
-                                 (int)threadIdx.x - 64, lin);
+                                 (int)threadIdx.x - 64);
         }
         continue;
       }
@@ -726,8 +629,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       if constexpr (EPI == EPI_ROWS) {
         const uint64_t addr = row_ok ? row_ptrs[t.row0 + r] : 0;
         epilogue_rows<OutT>(tbase, addr, col0, N, s_stage + q * ROWS_STAGE_BYTES, lane);
-      } else if constexpr (EPI == EPI_LINEAR) {
-        epilogue_linear<OutT>(tbase, t.g, t.row0 + r, row_ok, col0, N, C, lin);
       } else {
         OutT* crow = out_row(C, ldc, row_ptrs, t.row0 + r, row_ok);
         epilogue_tile<EPI, OutT>(tbase, crow, row_ok, col0, N);
@@ -754,10 +655,12 @@ __global__ void __launch_bounds__(THREADS, 1)
 // where A [M, Ktot] and B [N, Ktot] are K-major (the transposed routed rows: K runs over
 // the rows of all groups, grouped by expert).  Same pipeline as grouped_gemm_kernel
 // (TMA producer, single-thread tcgen05.mma issuer, double-buffered TMEM accumulators,
-// four epilogue warps); the tiles are 128 (M) x 256 (N) of one group.  Group starts must be multiples of BK (the dispatch plan's row_align 64): the
-// K tiles of a group then never reach into the next group, and every TMA K coordinate is
-// 16-byte aligned.  A start that is not is rounded down (wrong sums, no fault) and
+// four epilogue warps); the tiles are 128 (M) x 256 (N) of one group.  Group starts must
+// be multiples of BK (the dispatch plan's row_align 64): the K tiles of a group then never
+// reach into the next group, and every TMA K coordinate is 16-byte aligned.  A start that is not is rounded down (wrong sums, no fault) and
 // reported in the device error word.  A group without rows gets zeros.
+constexpr uint32_t kMnBox = 64 * BK * 2;  // one 64 x 64 MN-major box: 8 KB
+
 // Tile L -> (group, m0, n0), in bands of `band` m-tiles, m fastest inside a band: CTAs that
 // run at the same time then share the 256-wide B tiles, the larger operand of a tile, and
 // a band's A columns and the group's B rows stay in L2.
@@ -808,49 +711,16 @@ __device__ __forceinline__ void epilogue_f32_staged(uint32_t tbase, float* __res
   }
 }
 
-// Groups that start at any row (ANY, MN operands only): the K tiles of a group run from
-// its own first row -- rows are the outer coordinate of the TMA boxes, which needs no
-// alignment -- and the last one reaches up to 63 rows past its end, into the next group.
-// Those rows must not count, and they may hold anything (Inf and NaN times zero is not
-// zero), so the MMA warp overwrites them with zeros in both operands' boxes (a K row is 128
-// contiguous bytes of every box, whatever the swizzle) before lane 0 issues the tile's
-// MMAs, and it issues only the 16-row K steps that hold rows of the group: at most 15 rows
-// x 6 boxes x 128 bytes are written.  cmd: stage | valid rows << 8.  Lanes 1 to 31 wait for
-// it on the warp barrier (with all lanes following the pipeline's mbarriers instead, the
-// gradient of 8 x 14336 x 4096 weights took 2.06 ms against 1.82 at the power cap).
-__device__ __forceinline__ void zero_tile_rows(unsigned char* sA, unsigned char* sB, int cmd, int lane) {
-  const int stage = cmd & 255, valid = cmd >> 8;
-  const int n = ((valid + 15) / 16 * 16 - valid) * 8;  // 16-byte pieces per box
-#pragma unroll
-  for (int box = 0; box < 6; ++box) {
-    unsigned char* base = box < 2 ? sA + stage * A_BYTES + box * kMnBox : sB + stage * B_BYTES + (box - 2) * kMnBox;
-    for (int p = lane - 1; p < n; p += 31)
-      *reinterpret_cast<uint4*>(base + valid * 128 + p * 16) = make_uint4(0u, 0u, 0u, 0u);
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
-// A 16-bit tile row of zeros (a group without rows): this warp's 32 rows, all BN columns.
-template <typename OutT>
-__device__ __forceinline__ void store_zero_rows(uint64_t row_addr, int n0, int N, int lane) {
-  for (int i = 0; i < 32; ++i) {
-    const uint64_t dst = __shfl_sync(0xffffffffu, row_addr, i);
-    const int col = n0 + lane * 8;
-    if (dst != 0 && col < N) *reinterpret_cast<uint4*>(reinterpret_cast<OutT*>(dst) + col) = make_uint4(0u, 0u, 0u, 0u);
-  }
-}
-
 // MN = true: A and B are given as rows of K ([K, M] and [K, N], M / N contiguous: the
 // routed rows as they are) and are read as MN-major tiles -- TMA boxes of 64 MN-elements x
 // 64 K-rows, two for the 128 A columns and four for the 256 B columns of a tile, each box
 // one 8 KB region of 8 swizzle atoms along K -- instead of K-major boxes of transposed
 // copies.  MN = false: A [M, K] and B [N, K], K-major.
-template <typename OutT, bool MN, bool ANY = false>
+template <typename OutT, bool MN>
 __global__ void __launch_bounds__(THREADS, 1)
     wgrad_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       OutT* __restrict__ C, const int32_t* __restrict__ koff, int G, int M, int N, uint32_t idesc,
-                      int band, int k_rows) {
-  static_assert(!ANY || MN, "groups that start anywhere need row-major operands");
+                      int band) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -859,10 +729,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sB + STAGES * B_BYTES);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + NUM_BARS);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  [[maybe_unused]] volatile int* s_cmd = reinterpret_cast<volatile int*>(s_tmem + 2);  // ANY: rows to clear, -1: done
-  // first and end K tile of each group; ANY: its first row and end row
-  int* s_kb0 = reinterpret_cast<int*>(s_tmem + 4);
-  int* s_kb1 = s_kb0 + (MAX_GROUPS + 1);
+  int* s_kb0 = reinterpret_cast<int*>(s_tmem + 4);  // first K tile of each group
+  int* s_kb1 = s_kb0 + (MAX_GROUPS + 1);            // end K tile of each group
   // the epilogue warps' output stages (the launch requests SMEM_BYTES_ROWS)
   unsigned char* s_stage =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(s_kb1 + 2 * (MAX_GROUPS + 1)) + 15) & ~uintptr_t(15));
@@ -881,15 +749,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) *s_abort = 0;
   for (int g = threadIdx.x; g < G; g += blockDim.x) {
-    if constexpr (ANY) {
-      s_kb0[g] = min(max(koff[g], 0), k_rows);
-      s_kb1[g] = min(max(koff[g + 1], s_kb0[g]), k_rows);
-    } else {
-      const int a = max(koff[g], 0), b = max(koff[g + 1], a);
-      if (a % BK != 0) set_device_error(kErrBadGroupStart);
-      s_kb0[g] = a / BK;                    // rounded down: a K coordinate stays aligned
-      s_kb1[g] = (b + BK - 1) / BK;
-    }
+    const int a = max(koff[g], 0), b = max(koff[g + 1], a);
+    if (a % BK != 0) set_device_error(kErrBadGroupStart);
+    s_kb0[g] = a / BK;                    // rounded down: a K coordinate stays aligned
+    s_kb1[g] = (b + BK - 1) / BK;
   }
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -921,23 +784,21 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int L = blockIdx.x; L < total && ok; L += gridDim.x) {
         int g, m0, n0;
         wgrad_tile(L, MT, NB, band, g, m0, n0);
-        constexpr int STEP = ANY ? BK : 1;
-        for (int kb = s_kb0[g]; kb < s_kb1[g]; kb += STEP) {
-          const int k0 = ANY ? kb : kb * BK;
+        for (int kb = s_kb0[g]; kb < s_kb1[g]; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1, s_abort)) { ok = false; break; }
           const uint32_t fb = full_bar(stage);
           mbar_arrive_expect_tx(fb, STAGE_BYTES);
           const uint32_t a_dst = smem_u32(sA + stage * A_BYTES);
           const uint32_t b_dst = smem_u32(sB + stage * B_BYTES);
           if constexpr (MN) {
-            tma_load_2d(a_dst, &tmA, fb, m0, k0);
-            tma_load_2d(a_dst + kMnBox, &tmA, fb, m0 + 64, k0);
+            tma_load_2d(a_dst, &tmA, fb, m0, kb * BK);
+            tma_load_2d(a_dst + kMnBox, &tmA, fb, m0 + 64, kb * BK);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tma_load_2d(b_dst + i * kMnBox, &tmB, fb, n0 + 64 * i, k0);
+            for (int i = 0; i < 4; ++i) tma_load_2d(b_dst + i * kMnBox, &tmB, fb, n0 + 64 * i, kb * BK);
           } else {
-            tma_load_2d(a_dst, &tmA, fb, k0, m0);
-            tma_load_2d(b_dst, &tmB, fb, k0, n0);
-            tma_load_2d(b_dst + B_BYTES / 2, &tmB, fb, k0, n0 + 128);
+            tma_load_2d(a_dst, &tmA, fb, kb * BK, m0);
+            tma_load_2d(b_dst, &tmB, fb, kb * BK, n0);
+            tma_load_2d(b_dst + B_BYTES / 2, &tmB, fb, kb * BK, n0 + 128);
           }
           ++issued;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -964,25 +825,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1, s_abort)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-        constexpr int STEP = ANY ? BK : 1;
-        for (int kb = kb0; kb < kb1; kb += STEP) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(full_bar(stage), phase, s_abort)) { ok = false; break; }
-          int steps = BK / 16;
-          if constexpr (ANY) {
-            const int valid = kb1 - kb;
-            if (valid < BK) {               // the group's last rows
-              steps = (valid + 15) / 16;
-              if (valid < 16 * steps) {     // wake the other lanes, wait for them
-                *s_cmd = stage | valid << 8;
-                __syncwarp();
-                __syncwarp();
-              }
-            }
-          }
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk) {
-            if (ANY && kk >= steps) break;
             uint64_t a_desc, b_desc;
             if constexpr (MN) {   // K step of 16 rows = two 1 KB atoms along K
               a_desc = umma_desc_mn_sw128(smem_u32(sA + stage * A_BYTES) + kk * 2048, kMnBox, 1024);
@@ -1001,24 +848,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
-      if constexpr (ANY) {                  // the other lanes may leave
-        *s_cmd = -1;
-        __syncwarp();
-      }
       umma_commit(mma_done_bar);
       mbar_wait_drain(mma_done_bar, 0);
-    } else if constexpr (ANY) {
-      // asleep on the warp barrier until lane 0 has rows to clear
-      while (true) {
-        __syncwarp();
-        const int cmd = *s_cmd;
-        if (cmd < 0) break;
-        zero_tile_rows(sA, sB, cmd, lane);
-        __syncwarp();
-      }
     }
   } else {
     // --------------------------------------------------------------- epilogue
+    static_assert(sizeof(OutT) == 4, "the weight gradients are stored in fp32");
     const int q = warp & 3;
     unsigned char* stage = s_stage + q * ROWS_STAGE_BYTES;
     int acc = 0;
@@ -1027,24 +862,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       int g, m0, n0;
       wgrad_tile(L, MT, NB, band, g, m0, n0);
       const uint32_t tq = tmem_base + ((uint32_t)(q * 32) << 16);
-      if constexpr (sizeof(OutT) == 2) {    // one rounding to 16 bits, rows staged as in EPI_ROWS
-        const int row = m0 + q * 32 + lane;
-        const uint64_t addr =
-            row < M ? reinterpret_cast<uint64_t>(C) + ((uint64_t)g * M + row) * (uint64_t)N * sizeof(OutT) : 0;
-        if (s_kb1[g] <= s_kb0[g]) {
-          store_zero_rows<OutT>(addr, n0, N, lane);
-          continue;
-        }
-        if (!mbar_wait(tfull_bar(acc), acc_phase, s_abort)) break;
-        tc_fence_after();
-        epilogue_rows<OutT>(tq + (uint32_t)(acc * BN), addr, n0, N, stage, lane);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(tempty_bar(acc));
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
-        continue;
-      }
       if (s_kb1[g] <= s_kb0[g]) {           // empty group: zero tile, no accumulator used
         epilogue_f32_staged(tq, reinterpret_cast<float*>(C), (int64_t)g * M, M, N, m0 + q * 32, n0, stage, lane,
                             true);

@@ -277,7 +277,7 @@ def grouped_linear(A: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, bias
         out = torch.empty((rows_cap, N), dtype=A.dtype, device=A.device)
     lib = L.load()
     with _on(A.device):
-        need = lib.smoe_grouped_linear_workspace_size(rows_cap, N, w_layout)
+        need = lib.smoe_grouped_linear_workspace_size(rows_cap, N, Kd, G, w_layout)
         ws = _workspace(A.device, need) if need else None
         L.check(lib.smoe_grouped_linear(L.ptr(A), L.ptr(W), w_layout, L.ptr(bias),
                                         L.dtype_code(bias.dtype) if bias is not None else dt, act, L.ptr(residual),
@@ -325,9 +325,13 @@ def linear_wgrad(dz: torch.Tensor, A: torch.Tensor, offsets: torch.Tensor,
     _group_offsets(offsets, G)
     od = A.dtype if out_dtype is None else out_dtype
     dW = torch.empty((G, N, Kd), dtype=od, device=A.device)
+    lib = L.load()
     with _on(A.device):
-        L.check(L.load().smoe_linear_wgrad(L.ptr(dz), L.ptr(A), dt, L.ptr(offsets), G, rows_cap, N, Kd, L.ptr(dW),
-                                           L.dtype_code(od), L.stream_handle(A.device)), "smoe_linear_wgrad")
+        need = lib.smoe_linear_wgrad_workspace_size(rows_cap, G, N, Kd)
+        ws = _workspace(A.device, need) if need else None
+        L.check(lib.smoe_linear_wgrad(L.ptr(dz), L.ptr(A), dt, L.ptr(offsets), G, rows_cap, N, Kd, L.ptr(dW),
+                                      L.dtype_code(od), L.ptr(ws), need, L.stream_handle(A.device)),
+                "smoe_linear_wgrad")
     return dW
 
 

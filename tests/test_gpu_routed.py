@@ -301,6 +301,8 @@ GROUPS = [  # sizes, K, N, rows before the first group, rows behind the last
     ([129, 255, 3], 72, 200, 1, 130),    # sizes off every tile
     ([513, 64, 200], 256, 512, 0, 0),
     ([37] * 16 + [0] * 48, 136, 8, 0, 0),
+    ([20, 0, 1500], 80, 72, 0, 0),       # weight gradient split along the rows, slices without any
+    ([300, 5, 0, 200, 17] * 4, 64, 1056, 0, 3),   # several tiles per block, narrow last column tile
     ([0, 0, 0], 64, 64, 0, 7),           # no rows at all
 ]
 

@@ -71,7 +71,7 @@ def test_linear_refusals(lib):
     for bad in (dict(dt=F32), dict(db=P, bdt=1), dict(N=12), dict(G=1025), dict(dout=P + 2), dict(z=P + 2), dict(dz=P + 2)):
         assert act(**bad) == -4, bad
     assert act(db=P) == -5 and act(R=0) == 0 and act(act=0) == 0
-    wg = lambda **a: lib.smoe_linear_wgrad(*{**dict(dz=P, A=P, dt=BF, off=P, G=2, R=30, N=16, K=16, dW=P, odt=BF, st=None),  # noqa: E731
+    wg = lambda **a: lib.smoe_linear_wgrad(*{**dict(dz=P, A=P, dt=BF, off=P, G=2, R=30, N=16, K=16, dW=P, odt=BF, ws=None, wsb=0, st=None),  # noqa: E731
                                              **a}.values())
     for bad in (dict(G=0), dict(N=0), dict(K=0), dict(R=-1), dict(dz=None), dict(A=None), dict(off=None), dict(dW=None)):
         assert wg(**bad) == -1, bad
@@ -80,11 +80,14 @@ def test_linear_refusals(lib):
 
 
 def test_workspace_sizes(lib):
-    # split-K scratch only where the launch can have few tiles
-    assert lib.smoe_grouped_linear_workspace_size(2, 4096, L.SMOE_W_NK) == 0       # decode kernel
-    assert lib.smoe_grouped_linear_workspace_size(2, 4096, L.SMOE_W_KN) > 0
-    assert lib.smoe_grouped_linear_workspace_size(64, 4096, L.SMOE_W_NK) > 0
-    assert lib.smoe_grouped_linear_workspace_size(16384, 4096, L.SMOE_W_NK) == 0
+    # partial tiles only where a launch can have few of them
+    assert lib.smoe_grouped_linear_workspace_size(2, 4096, 4096, 8, L.SMOE_W_NK) == 0       # decode kernel
+    assert lib.smoe_grouped_linear_workspace_size(2, 4096, 4096, 8, L.SMOE_W_KN) > 0
+    assert 0 < lib.smoe_grouped_linear_workspace_size(64, 4096, 4096, 1, L.SMOE_W_NK) <= 64 << 20
+    assert lib.smoe_grouped_linear_workspace_size(64, 4096, 128, 1, L.SMOE_W_NK) == 0       # short K
+    assert lib.smoe_grouped_linear_workspace_size(16384, 4096, 4096, 8, L.SMOE_W_NK) == 0
+    assert 0 < lib.smoe_linear_wgrad_workspace_size(32768, 1, 512, 512) <= 64 << 20
+    assert lib.smoe_linear_wgrad_workspace_size(16384, 8, 14336, 4096) == 0
     # bias partials: a row per slice (16 to 512 rows) and one per group
     assert lib.smoe_linear_act_bwd_workspace_size(64, 8, 4) == (4 + 4) * 8 * 4
     assert lib.smoe_linear_act_bwd_workspace_size(1 << 20, 8, 4) == ((1 << 20) // 512 + 4) * 8 * 4
