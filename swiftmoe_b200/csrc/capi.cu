@@ -631,7 +631,8 @@ SplitPlan linear_split_plan(int64_t rows_cap, int N, int K, int G) {
   const int64_t even = groups * cdiv(cdiv(rows_cap, groups), lin::BM) * nb, one = cdiv(rows_cap, lin::BM) * nb;
   const int kb = (int)cdiv(K, lin::BK);
   for (int64_t tiles : {even, one})
-    if (lin::split_units(tiles, kb, p.rows, device_sms(), slots) > 1) p.slots = (int)slots;
+    if (tiles <= slots && lin::split_units((uint32_t)tiles, kb, p.rows, device_sms(), (uint32_t)slots) > 1)
+      p.slots = (int)slots;
   return p;
 }
 
@@ -672,7 +673,8 @@ int linear_gemm_t(const void* A, const void* B, void* C, const int32_t* offsets,
 int wgrad_slices(int64_t rows_cap, int G, int N, int K) {
   const int64_t tiles = (int64_t)G * cdiv(N, lin::BM) * cdiv(K, lin::BN);
   const int kb = (int)cdiv(cdiv(rows_cap, G), lin::BK);
-  return lin::split_units(tiles, kb, lin::BM, device_sms(), kSplitBytes / (lin::BM * lin::BN * 4));
+  constexpr int slots = (int)(kSplitBytes / (lin::BM * lin::BN * 4));
+  return tiles <= slots ? lin::split_units((uint32_t)tiles, kb, lin::BM, device_sms(), slots) : 1;
 }
 
 template <typename OutT>

@@ -205,18 +205,30 @@ __device__ __forceinline__ void epilogue_tile(uint32_t tbase, int g, int row, in
                                              : make_uint4(0u, 0u, 0u, 0u);
       }
     }
-    float bias[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) bias[j] = 0.f;
-    if (lin.bias != nullptr)
+    uint4 bias[4];
+    const bool bias16 = lin.bias != nullptr && !lin.bias_f32;
+    if (bias16)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (col + 8 * j < N)
-          add_bias<T>(lin, (int64_t)g * N + col + 8 * j, reinterpret_cast<float(&)[8]>(bias[8 * j]));
+        bias[j] = col + 8 * j < N
+                      ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(lin.bias) + (int64_t)g * N + col) + j)
+                      : make_uint4(0u, 0u, 0u, 0u);
     tmem_ld_wait();
     float f[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) + bias[j];
+    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+    if (bias16) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const T* e = reinterpret_cast<const T*>(&bias[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[8 * j + i] += Num<T>::to_f(e[i]);
+      }
+    } else if (lin.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + 8 * j < N) add_bias<T>(lin, (int64_t)g * N + col + 8 * j, reinterpret_cast<float(&)[8]>(f[8 * j]));
+    }
     uint4 u[4];
     if (lin.preact != nullptr) {
       pack_cols<T, 32>(f, u);
@@ -262,16 +274,17 @@ __device__ __forceinline__ void fill_other_rows(const LinearEpi& lin, T* __restr
 // fill the ring and drain the tile, and for its partial tile's way out and back 8 blocks'
 // time per 128 rows; the second launch counts 6.  Both launches compute it from the same
 // numbers.  rows: rows of a slot.
-__host__ __device__ inline int split_units(int64_t tiles, int kb, int rows, int ctas, int64_t slots) {
+// (32-bit divisions: one thread of every block works this out before the block can start.)
+__host__ __device__ inline int split_units(uint32_t tiles, uint32_t kb, uint32_t rows, uint32_t ctas, uint32_t slots) {
   int best = 1;
-  int64_t best_cost = INT64_MAX;
-  for (int ks = 1; ks <= MAX_SPLIT; ++ks) {
-    if (ks > 1 && (tiles * ks > slots || kb / ks < 4)) break;
-    const int64_t waves = (tiles * ks + ctas - 1) / ctas;
-    const int64_t cost = waves * (((kb + ks - 1) / ks + 3) * 16 + (ks > 1 ? rows : 0)) + (ks > 1 ? 6 * 16 : 0);
+  uint64_t best_cost = ~0ull;
+  for (uint32_t ks = 1; ks <= MAX_SPLIT; ++ks) {
+    if (ks > 1 && (tiles > slots / ks || kb < 4 * ks)) break;
+    const uint32_t waves = (tiles * ks + ctas - 1) / ctas, blocks = (kb + ks - 1) / ks + 3;
+    const uint64_t cost = (uint64_t)waves * (blocks * 16 + (ks > 1 ? rows : 0)) + (ks > 1 ? 6 * 16 : 0);
     if (cost < best_cost) {
       best_cost = cost;
-      best = ks;
+      best = (int)ks;
     }
   }
   return best;
@@ -296,7 +309,7 @@ __device__ __forceinline__ void sum_partials(const float* ws, int64_t first, int
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = 0.f;
   const float* p = ws + first * rows * BN + ((int64_t)2 * p8 * rows + r) * 4;
-#pragma unroll 4
+#pragma unroll 8
   for (int q = 0; q < n; ++q, p += (int64_t)rows * BN) {
     const float4 a = __ldcg(reinterpret_cast<const float4*>(p));
     const float4 b = __ldcg(reinterpret_cast<const float4*>(p + rows * 4));
@@ -335,12 +348,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 2) tc::scan_group_table(G, s_ts);
+  if (warp == 2) {
+    tc::scan_group_table(G, s_ts);
+    if (lane == 0) *sm.word = ws != nullptr ? split_units(s_ts[G], KB, slot_rows, gridDim.x, slots) : 1;
+  }
   __syncthreads();
   const uint32_t tmem_base = *sm.tmem;
-  const int tiles = s_ts[G];
-  const int ks_n = ws != nullptr ? split_units(tiles, KB, slot_rows, gridDim.x, slots) : 1;
-  const int total = tiles * ks_n;
+  const int ks_n = *sm.word, total = s_ts[G] * ks_n;
   auto tile_of = [&](int L) { return tc::decode_tile_t<BM>(L / ks_n, s_ts, s_beg, s_fin, G, NB, gm); };
 
   if (warp == 0 || warp == WARP_B) {
@@ -461,14 +475,16 @@ __global__ void __launch_bounds__(256) linear_sum_kernel(T* __restrict__ C, cons
                                                          const float* __restrict__ ws, int slots, int slot_rows,
                                                          int ctas) {
   pdl_wait_and_release();
-  __shared__ int s_beg[MAX_GROUPS + 1], s_fin[MAX_GROUPS + 1], s_ts[MAX_GROUPS + 1];
+  __shared__ int s_beg[MAX_GROUPS + 1], s_fin[MAX_GROUPS + 1], s_ts[MAX_GROUPS + 1], s_ks;
   const int NB = (N + BN - 1) / BN, KB = (K + BK - 1) / BK;
   tc::load_group_table<BM>(offsets, nullptr, G, rows_cap, NB, s_beg, s_fin, s_ts);
   __syncthreads();
-  if (threadIdx.x < 32) tc::scan_group_table(G, s_ts);
+  if (threadIdx.x < 32) {
+    tc::scan_group_table(G, s_ts);
+    if (threadIdx.x == 0) s_ks = split_units(s_ts[G], KB, slot_rows, ctas, slots);
+  }
   __syncthreads();
-  const int tiles = s_ts[G];
-  const int ks_n = split_units(tiles, KB, slot_rows, ctas, slots);
+  const int tiles = s_ts[G], ks_n = s_ks;
   if (ks_n == 1) return;
   const int per = slot_rows * (BN / 8);  // (8 columns, row) pairs of a tile, rows fastest
   const int64_t total = (int64_t)tiles * per;
