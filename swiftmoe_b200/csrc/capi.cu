@@ -368,7 +368,7 @@ int launch_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, float* C, const i
 template <int EPI, typename T, typename OutT>
 int launch_gemv_t(const void* A, const void* B, const void* B3, void* C, const uint64_t* row_ptrs,
                   const int32_t* offsets, const int32_t* ends, int G, int64_t rows_cap, int N, int K,
-                  cudaStream_t st, const int32_t* a_index, int a_rows, const LinearEpi& lin = LinearEpi()) {
+                  cudaStream_t st, const int32_t* a_index, int a_rows) {
   // one warp (two for rows of 8192 or more elements) per (group with rows, column); at
   // most min(G, rows_cap) groups have rows.  Measured on the Mixtral decode shapes: two
   // warps take the 14336-element down rows in 54 us (one: 60, four: 57); the 4096-element
@@ -379,13 +379,13 @@ int launch_gemv_t(const void* A, const void* B, const void* B3, void* C, const u
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv(cols, CPB), 65535));
     SMOE_CK(launch_k(gemv::grouped_gemv_kernel<EPI, T, OutT, 2>, grid, gemv::THREADS, 0, st, 
         (const T*)A, (const T*)B, (const T*)B3, (OutT*)C, N, row_ptrs, offsets, ends, G, N, K, (int)rows_cap, a_index,
-        a_rows, lin));
+        a_rows));
   } else {
     const unsigned grid = (unsigned)std::max<int64_t>(
         1, std::min<int64_t>(cdiv(cols * 32, gemv::THREADS), (int64_t)device_sms() * 8));
     SMOE_CK(launch_k(gemv::grouped_gemv_kernel<EPI, T, OutT, 1>, grid, gemv::THREADS, 0, st, 
         (const T*)A, (const T*)B, (const T*)B3, (OutT*)C, N, row_ptrs, offsets, ends, G, N, K, (int)rows_cap, a_index,
-        a_rows, lin));
+        a_rows));
   }
   SMOE_CK(cudaGetLastError());
   return SMOE_OK;
@@ -640,13 +640,24 @@ SplitPlan linear_split_plan(int64_t rows_cap, int N, int K, int G) {
 // whole expert, longer ones half as high.
 int linear_band(int K) { return K <= 4096 ? 32 : tc::GM_DEFAULT; }
 
+// Decode: one or two rows (whose shared-memory copy still leaves two blocks per SM).
+bool linear_gemv_rows(int64_t rows_cap, int K) { return rows_cap <= lin::GEMV_ROWS && rows_cap * K * 2 <= 100 << 10; }
+
 template <typename T, bool BMN>
 int linear_gemm_t(const void* A, const void* B, void* C, const int32_t* offsets, int G, int64_t rows_cap, int N, int K,
                   const LinearEpi& epi, void* workspace, size_t workspace_bytes, cudaStream_t st) {
   constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
-  if (!BMN && rows_cap <= gemv::DISPATCH_ROWS)  // decode: the weights of the groups with rows, streamed once
-    return launch_gemv_t<gemv::EPI_LINEAR, T, T>(A, B, nullptr, C, nullptr, offsets, nullptr, G, rows_cap, N, K, st,
-                                                 nullptr, (int)rows_cap, epi);
+  if (!BMN && linear_gemv_rows(rows_cap, K)) {
+    static SmemGrant done_v;
+    auto kern_v = lin::linear_gemv_kernel<T>;
+    const int smem = (int)(rows_cap * K * 2);
+    SMOE_CK(ensure_smem(kern_v, smem, &done_v));
+    const int64_t tasks = std::min<int64_t>(G, rows_cap) * N;
+    const unsigned grid_v = (unsigned)std::min<int64_t>(cdiv(tasks, lin::GEMV_THREADS / 32), (int64_t)device_sms() * 2);
+    SMOE_CK(launch_k(kern_v, grid_v, lin::GEMV_THREADS, smem, st, (const T*)A, (const T*)B, (T*)C, offsets, G, N, K,
+                     (int)rows_cap, epi));
+    return SMOE_OK;
+  }
   const SplitPlan sp = linear_split_plan(rows_cap, N, K, G);
   if (sp.slots > 0 && (!workspace || workspace_bytes < sp.bytes())) return SMOE_ERR_WORKSPACE;
   float* ws = sp.slots > 0 ? static_cast<float*>(workspace) : nullptr;
@@ -1194,7 +1205,7 @@ int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const fl
 #undef SMOE_ROWS_CASE
 
 size_t smoe_grouped_linear_workspace_size(int64_t rows_cap, int N, int K, int G, int w_layout) {
-  if (rows_cap < 1 || N < 1 || K < 1 || G < 1 || (w_layout == SMOE_W_NK && rows_cap <= gemv::DISPATCH_ROWS)) return 0;
+  if (rows_cap < 1 || N < 1 || K < 1 || G < 1 || (w_layout == SMOE_W_NK && linear_gemv_rows(rows_cap, K))) return 0;
   return linear_split_plan(rows_cap, N, K, G).bytes();
 }
 

@@ -20,7 +20,6 @@
 // gathers the token rows itself, no permuted copy); an index outside [0, a_rows) reads
 // zeros.
 #pragma once
-#include "activation.cuh"
 #include "common.cuh"
 
 namespace smoe {
@@ -56,10 +55,6 @@ __device__ __forceinline__ float warp_sum(float v) {
 // K, and the slices' sums are added in slice order (deterministic).  KS = 2 for long rows
 // (the down projection's 28 KB rows): half the load rounds per task and twice the tasks,
 // so the last wave of tasks is shorter.
-// EPI_LINEAR (the grouped linear layers): lane 0 adds bias, activation and residual to the
-// column's sum; the rows of no group are filled by the first blocks when lin.fill is set.
-constexpr int EPI_LINEAR = 4;
-
 template <int EPI, typename T, typename OutT, int KS>
 __global__ void __launch_bounds__(THREADS, 2) grouped_gemv_kernel(const T* __restrict__ A, const T* __restrict__ B,
                                                                const T* __restrict__ B3, OutT* __restrict__ C,
@@ -67,7 +62,7 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_gemv_kernel(const T* __res
                                                                const int32_t* __restrict__ offsets,
                                                                const int32_t* __restrict__ ends, int G, int N, int K,
                                                                int rows_cap, const int32_t* __restrict__ a_index,
-                                                               int a_rows, const LinearEpi lin) {
+                                                               int a_rows) {
   pdl_wait_and_release();
   constexpr int CPB = (THREADS / 32) / KS;   // columns per block and step
   constexpr int H = EPI == SMOE_EPI_SWIGLU ? 2 : 1;
@@ -94,16 +89,6 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_gemv_kernel(const T* __res
     if (threadIdx.x == 0) s_nact = n;
   }
   __syncthreads();
-  if constexpr (EPI == EPI_LINEAR) {
-    if (lin.fill) {  // rows of no group: the residual, or zeros
-      const int64_t first = s_beg[0], last = s_fin[G - 1];
-      const int64_t head = first * N, total = head + ((int64_t)rows_cap - last) * N;
-      for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t p = i < head ? i : last * N + (i - head);
-        C[p] = lin.residual != nullptr ? static_cast<const OutT*>(lin.residual)[p] : Num<OutT>::from_f(0.f);
-      }
-    }
-  }
   const int lane = threadIdx.x & 31;
   const int wib = threadIdx.x >> 5;          // warp in block
   const int slot = wib / KS, part = wib - (wib / KS) * KS;
@@ -180,17 +165,6 @@ __global__ void __launch_bounds__(THREADS, 2) grouped_gemv_kernel(const T* __res
           float out = v[r][0];
           if (EPI == SMOE_EPI_SWIGLU) out = out / (1.0f + __expf(-out)) * v[r][H - 1];
           const int row = b + r;
-          if constexpr (EPI == EPI_LINEAR) {
-            const int64_t at = (int64_t)row * N + n;
-            if (lin.bias != nullptr)
-              out += lin.bias_f32 ? static_cast<const float*>(lin.bias)[(int64_t)g * N + n]
-                                  : Num<OutT>::to_f(static_cast<const OutT*>(lin.bias)[(int64_t)g * N + n]);
-            if (lin.preact != nullptr) static_cast<OutT*>(lin.preact)[at] = Num<OutT>::from_f(out);
-            float z[1] = {out};
-            apply_act(lin.act, z);
-            out = z[0];
-            if (lin.residual != nullptr) out += Num<OutT>::to_f(static_cast<const OutT*>(lin.residual)[at]);
-          }
           OutT* crow = row_ptrs ? reinterpret_cast<OutT*>(row_ptrs[row]) : C + (int64_t)row * ldc;
           if (crow != nullptr) crow[n] = Num<OutT>::from_f(out);
         }
