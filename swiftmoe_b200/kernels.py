@@ -25,10 +25,21 @@ def _workspace(device, nbytes: int) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
 
 
-def _same_device(device, *ts):
+def _device_of(first: torch.Tensor, *ts) -> torch.device:
+    """The CUDA device of ``first``, on which all of ``ts`` (None: absent) must be, contiguous.
+    (One pass over the tensors: these checks are a good part of a small call's host time.)"""
+    dev = first.device
+    if not first.is_cuda:
+        raise L.SwiftMoEError("swiftmoe_b200 kernels need CUDA tensors (no CPU fallback)")
+    if not first.is_contiguous():
+        raise L.SwiftMoEError("swiftmoe_b200 kernels need contiguous tensors")
     for t in ts:
-        if t is not None and t.device != device:
-            raise L.SwiftMoEError(f"tensors on different devices: {device} and {t.device}")
+        if t is not None:
+            if t.device != dev:
+                raise L.SwiftMoEError(f"tensors on different devices: {dev} and {t.device}")
+            if not t.is_contiguous():
+                raise L.SwiftMoEError("swiftmoe_b200 kernels need contiguous tensors")
+    return dev
 
 
 _HERE = nullcontext()
@@ -128,18 +139,17 @@ def combine(y: torch.Tensor, slot_row: torch.Tensor, w: torch.Tensor, T: int, k:
     return out
 
 
-def _plan_args(plan: dict, rows: int, device, w: Optional[torch.Tensor]):
-    """(slot_row, T, k) of a dispatch plan after checking that it fits `rows` rows and w."""
-    slot_row, T, k = plan["slot_row"], plan["T"], plan["k"]
-    _need_cuda(slot_row, plan["offsets"], w)
-    _same_device(device, slot_row, plan["offsets"], w)
-    if slot_row.dtype != torch.int32 or plan["offsets"].dtype != torch.int32 or slot_row.numel() != T * k:
+def _plan_args(plan: dict, rows: int, w: Optional[torch.Tensor]):
+    """(slot_row, offsets, T, k) of a dispatch plan after checking that it fits `rows` rows
+    and w."""
+    slot_row, offsets, T, k = plan["slot_row"], plan["offsets"], plan["T"], plan["k"]
+    if slot_row.dtype != torch.int32 or offsets.dtype != torch.int32 or slot_row.numel() != T * k:
         raise L.SwiftMoEError("not a dispatch plan: slot_row must be int32 [T*k], offsets int32")
     if rows < plan["rows_cap"]:
         raise L.SwiftMoEError(f"the plan has up to {plan['rows_cap']} rows, the tensor only {rows}")
-    if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (T, k)):
+    if w is not None and (w.dtype != torch.float32 or w.shape != (T, k)):
         raise L.SwiftMoEError(f"weights must be float32 [{T}, {k}], got {w.dtype} {tuple(w.shape)}")
-    return slot_row, T, k
+    return slot_row, offsets, T, k
 
 
 def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, rows_cap: Optional[int] = None,
@@ -150,34 +160,31 @@ def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, 
     With ``y`` [rows_cap, d] (needs w) returns (rows, dw [T,k] fp32), dw[t,j] = <x[t],
     y[slot_row[t,j]]>: for x = the gradient of ``unsort_rows``' output and y = its rows
     these are its gradients."""
-    _need_cuda(x, y)
     rows_cap = plan["rows_cap"] if rows_cap is None else rows_cap
-    slot_row, T, k = _plan_args(plan, rows_cap, x.device, w)
+    slot_row, offsets, T, k = _plan_args(plan, rows_cap, w)
     row_token = plan["row_token"] if plan.get("row_align") != 1 else None
-    _need_cuda(row_token)
-    _same_device(x.device, y, row_token)
+    dev = _device_of(x, slot_row, offsets, row_token, w, y)
     if x.dim() != 2 or x.shape[0] != T:
         raise L.SwiftMoEError(f"the plan is for {T} tokens, got x of shape {tuple(x.shape)}")
     if row_token is not None and (row_token.dtype != torch.int32 or row_token.numel() < plan["rows_cap"]):
         raise L.SwiftMoEError("not a dispatch plan: row_token must be int32 [rows_cap]")
     d = x.shape[1]
-    if y is not None and (w is None or y.dtype != x.dtype or tuple(y.shape) != (rows_cap, d)):
+    if y is not None and (w is None or y.dtype != x.dtype or y.shape != (rows_cap, d)):
         raise L.SwiftMoEError("y needs weights, x's dtype and shape [rows_cap, d]")
-    rows = torch.empty((rows_cap, d), dtype=x.dtype, device=x.device)
-    dw = torch.empty((T, k), dtype=torch.float32, device=x.device) if y is not None else None
-    with _on(x.device):
-        L.check(L.load().smoe_sort_rows(L.ptr(x), L.dtype_code(x.dtype), L.ptr(slot_row), L.ptr(w), T, k, d,
-                                        L.ptr(row_token), L.ptr(plan["offsets"]), plan["offsets"].numel() - 1, rows_cap,
-                                        L.ptr(rows), L.ptr(y), L.ptr(dw), L.stream_handle(x.device)), "smoe_sort_rows")
+    dt = L.dtype_code(x.dtype)
+    rows = torch.empty((rows_cap, d), dtype=x.dtype, device=dev)
+    dw = torch.empty((T, k), dtype=torch.float32, device=dev) if y is not None else None
+    with _on(dev):
+        L.check(L.load().smoe_sort_rows(x.data_ptr(), dt, slot_row.data_ptr(), L.ptr(w), T, k, d, L.ptr(row_token),
+                                        offsets.data_ptr(), offsets.numel() - 1, rows_cap, rows.data_ptr(), L.ptr(y),
+                                        L.ptr(dw), L.stream_handle(dev)), "smoe_sort_rows")
     return rows if y is None else (rows, dw)
 
 
 def sort_tokens(x: torch.Tensor, idx: torch.Tensor, num_experts: int, w: Optional[torch.Tensor] = None,
                 capacity: int = 0, row_align: int = 1):
     """(rows, plan): ``dispatch_plan`` and ``sort_rows`` in one library call."""
-    _need_cuda(x, idx, w)
-    dev = x.device
-    _same_device(dev, idx, w)
+    dev = _device_of(x, idx, w)
     if idx.dtype != torch.int32 or idx.dim() != 2:
         raise L.SwiftMoEError("idx must be int32 [T, k]")
     T, k = idx.shape
@@ -188,11 +195,12 @@ def sort_tokens(x: torch.Tensor, idx: torch.Tensor, num_experts: int, w: Optiona
     dt, d, E, lib, i32 = L.dtype_code(x.dtype), x.shape[1], num_experts, L.load(), torch.int32
     rows_cap = lib.smoe_plan_rows_cap(T, k, E, capacity, row_align)
     need = lib.smoe_plan_workspace_size(T, k, E)
-    counts = torch.empty(max(E, 0), dtype=i32, device=dev)
-    offsets = torch.empty(max(E, 0) + 1, dtype=i32, device=dev)
-    slot_row = torch.empty(T * k, dtype=i32, device=dev)
-    row_token = torch.empty(max(rows_cap, 1), dtype=i32, device=dev)
-    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+    if E < 1:
+        raise L.SwiftMoEError("num_experts must be positive")
+    # the plan's arrays and its scratch from one allocation
+    counts, offsets, slot_row, row_token, ws = torch.empty(
+        2 * E + 1 + T * k + max(rows_cap, 1) + (need + 3) // 4, dtype=i32, device=dev).split_with_sizes(
+        (E, E + 1, T * k, max(rows_cap, 1), (need + 3) // 4))
     rows = torch.empty((rows_cap, d), dtype=x.dtype, device=dev)
     with _on(dev):
         L.check(lib.smoe_sort_tokens(x.data_ptr(), dt, idx.data_ptr(), L.ptr(w), T, k, d, E, capacity, row_align,
@@ -211,23 +219,23 @@ def unsort_rows(y: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, r
     With ``x`` [T, d] (needs w) returns (out, dw [T,k] fp32), dw[t,j] = <x[t],
     y[slot_row[t,j]]>: for y = the gradient of ``sort_rows``' rows and x = its input these
     are its gradients."""
-    _need_cuda(y, residual, x)
-    _same_device(y.device, residual, x)
     if y.dim() != 2:
         raise L.SwiftMoEError(f"rows must be [rows, d], got {tuple(y.shape)}")
     rows_cap, d = y.shape
-    slot_row, T, k = _plan_args(plan, rows_cap, y.device, w)
+    slot_row, _, T, k = _plan_args(plan, rows_cap, w)
+    dev = _device_of(y, slot_row, w, residual, x)
     for name, t in (("residual", residual), ("x", x)):
-        if t is not None and (t.dtype != y.dtype or tuple(t.shape) != (T, d)):
+        if t is not None and (t.dtype != y.dtype or t.shape != (T, d)):
             raise L.SwiftMoEError(f"{name} must be {y.dtype} [{T}, {d}], got {t.dtype} {tuple(t.shape)}")
     if x is not None and w is None:
         raise L.SwiftMoEError("the weights' gradient needs the weights")
-    out = torch.empty((T, d), dtype=y.dtype, device=y.device)
-    dw = torch.empty((T, k), dtype=torch.float32, device=y.device) if x is not None else None
-    with _on(y.device):
-        L.check(L.load().smoe_unsort_rows(L.ptr(y), L.dtype_code(y.dtype), L.ptr(slot_row), L.ptr(w), T, k, d, rows_cap,
-                                          L.ptr(residual), L.ptr(out), L.ptr(x), L.ptr(dw),
-                                          L.stream_handle(y.device)), "smoe_unsort_rows")
+    dt = L.dtype_code(y.dtype)
+    out = torch.empty((T, d), dtype=y.dtype, device=dev)
+    dw = torch.empty((T, k), dtype=torch.float32, device=dev) if x is not None else None
+    with _on(dev):
+        L.check(L.load().smoe_unsort_rows(y.data_ptr(), dt, slot_row.data_ptr(), L.ptr(w), T, k, d, rows_cap,
+                                          L.ptr(residual), out.data_ptr(), L.ptr(x), L.ptr(dw), L.stream_handle(dev)),
+                "smoe_unsort_rows")
     return out if x is None else (out, dw)
 
 
@@ -257,8 +265,7 @@ def grouped_linear(A: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, bias
     offsets[g+1]); W [G, N, K] (``L.SMOE_W_KN``: [G, K, N], C = A W_g), bias [G, N] in A's dtype
     or fp32.  Rows of no group become the residual alone (zeros without one); given ``out``,
     its rows of no group stay as they were.  ``preact`` [rows, N] receives A W_g^T + bias[g]."""
-    _need_cuda(A, W, offsets, bias, residual, preact, out)
-    _same_device(A.device, W, offsets, bias, residual, preact, out)
+    dev = _device_of(A, W, offsets, bias, residual, preact, out)
     act, dt = _act_code(activation), _linear_dtype(A)
     if A.dim() != 2 or W.dim() != 3 or W.dtype != A.dtype:
         raise L.SwiftMoEError("A must be [rows, K], W [G, N, K] of the same dtype")
@@ -267,22 +274,22 @@ def grouped_linear(A: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, bias
     if K2 != Kd:
         raise L.SwiftMoEError("K mismatch")
     _group_offsets(offsets, G)
-    if bias is not None and (tuple(bias.shape) != (G, N) or bias.dtype not in (A.dtype, torch.float32)):
+    if bias is not None and (bias.shape != (G, N) or bias.dtype not in (A.dtype, torch.float32)):
         raise L.SwiftMoEError(f"bias must be {A.dtype} or float32 [{G}, {N}], got {bias.dtype} {tuple(bias.shape)}")
     for name, t in (("residual", residual), ("preact", preact), ("out", out)):
-        if t is not None and (t.dtype != A.dtype or tuple(t.shape) != (rows_cap, N)):
+        if t is not None and (t.dtype != A.dtype or t.shape != (rows_cap, N)):
             raise L.SwiftMoEError(f"{name} must be {A.dtype} [{rows_cap}, {N}], got {t.dtype} {tuple(t.shape)}")
     fill = out is None
     if out is None:
-        out = torch.empty((rows_cap, N), dtype=A.dtype, device=A.device)
+        out = torch.empty((rows_cap, N), dtype=A.dtype, device=dev)
     lib = L.load()
-    with _on(A.device):
+    with _on(dev):
         need = lib.smoe_grouped_linear_workspace_size(rows_cap, N, Kd, G, w_layout)
-        ws = _workspace(A.device, need) if need else None
-        L.check(lib.smoe_grouped_linear(L.ptr(A), L.ptr(W), w_layout, L.ptr(bias),
-                                        L.dtype_code(bias.dtype) if bias is not None else dt, act, L.ptr(residual),
-                                        L.ptr(preact), int(fill), L.ptr(out), dt, L.ptr(offsets), G, rows_cap, N, Kd,
-                                        L.ptr(ws), need, L.stream_handle(A.device)), "smoe_grouped_linear")
+        ws = _workspace(dev, need) if need else None
+        L.check(lib.smoe_grouped_linear(A.data_ptr(), W.data_ptr(), w_layout, L.ptr(bias),
+                                        dt if bias is None or bias.dtype == A.dtype else L.SMOE_F32, act,
+                                        L.ptr(residual), L.ptr(preact), fill, out.data_ptr(), dt, offsets.data_ptr(), G,
+                                        rows_cap, N, Kd, L.ptr(ws), need, L.stream_handle(dev)), "smoe_grouped_linear")
     return out
 
 
@@ -290,8 +297,7 @@ def linear_act_bwd(dout: torch.Tensor, offsets: torch.Tensor, activation: str, p
                    bias_dtype: Optional[torch.dtype] = None):
     """(dz, dbias): dz = dout * act'(preact) for the rows of the groups (dout itself for "none"),
     dbias [G, N] = the groups' column sums of the unrounded dz, or None without bias_dtype."""
-    _need_cuda(dout, offsets, preact)
-    _same_device(dout.device, offsets, preact)
+    dev = _device_of(dout, offsets, preact)
     act, dt = _act_code(activation), _linear_dtype(dout)
     rows_cap, N = dout.shape
     G = offsets.numel() - 1
@@ -299,14 +305,14 @@ def linear_act_bwd(dout: torch.Tensor, offsets: torch.Tensor, activation: str, p
     if act and (preact is None or preact.dtype != dout.dtype or preact.shape != dout.shape):
         raise L.SwiftMoEError("preact must have dout's dtype and shape")
     dz = torch.empty_like(dout) if act else dout
-    dbias = torch.empty((G, N), dtype=bias_dtype, device=dout.device) if bias_dtype is not None else None
+    dbias = torch.empty((G, N), dtype=bias_dtype, device=dev) if bias_dtype is not None else None
     lib = L.load()
-    with _on(dout.device):
+    with _on(dev):
         need = lib.smoe_linear_act_bwd_workspace_size(rows_cap, N, G) if dbias is not None else 0
-        ws = _workspace(dout.device, need) if need else None
+        ws = _workspace(dev, need) if need else None
         L.check(lib.smoe_linear_act_bwd(L.ptr(dout), L.ptr(preact), act, L.ptr(dz), L.ptr(dbias),
                                         L.dtype_code(bias_dtype) if dbias is not None else dt, dt, L.ptr(offsets), G,
-                                        rows_cap, N, L.ptr(ws), need, L.stream_handle(dout.device)),
+                                        rows_cap, N, L.ptr(ws), need, L.stream_handle(dev)),
                 "smoe_linear_act_bwd")
     return dz, dbias
 
@@ -315,8 +321,7 @@ def linear_wgrad(dz: torch.Tensor, A: torch.Tensor, offsets: torch.Tensor,
                  out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """dW [G, N, K] = dz_g^T A_g over the rows of every group (any group starts), in A's dtype
     or fp32 (``out_dtype``); groups without rows get zeros."""
-    _need_cuda(dz, A, offsets)
-    _same_device(A.device, dz, offsets)
+    dev = _device_of(A, dz, offsets)
     dt = _linear_dtype(A)
     if dz.dtype != A.dtype or dz.dim() != 2 or A.dim() != 2 or dz.shape[0] != A.shape[0]:
         raise L.SwiftMoEError("dz [rows, N] and A [rows, K] must have the same rows and dtype")
@@ -324,13 +329,13 @@ def linear_wgrad(dz: torch.Tensor, A: torch.Tensor, offsets: torch.Tensor,
     Kd, G = A.shape[1], offsets.numel() - 1
     _group_offsets(offsets, G)
     od = A.dtype if out_dtype is None else out_dtype
-    dW = torch.empty((G, N, Kd), dtype=od, device=A.device)
+    dW = torch.empty((G, N, Kd), dtype=od, device=dev)
     lib = L.load()
-    with _on(A.device):
+    with _on(dev):
         need = lib.smoe_linear_wgrad_workspace_size(rows_cap, G, N, Kd)
-        ws = _workspace(A.device, need) if need else None
-        L.check(lib.smoe_linear_wgrad(L.ptr(dz), L.ptr(A), dt, L.ptr(offsets), G, rows_cap, N, Kd, L.ptr(dW),
-                                      L.dtype_code(od), L.ptr(ws), need, L.stream_handle(A.device)),
+        ws = _workspace(dev, need) if need else None
+        L.check(lib.smoe_linear_wgrad(dz.data_ptr(), A.data_ptr(), dt, offsets.data_ptr(), G, rows_cap, N, Kd,
+                                      dW.data_ptr(), L.dtype_code(od), L.ptr(ws), need, L.stream_handle(dev)),
                 "smoe_linear_wgrad")
     return dW
 

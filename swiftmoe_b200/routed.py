@@ -38,13 +38,13 @@ class _SortTokens(torch.autograd.Function):
         rows, plan = K.sort_tokens(x, args[0], args[1], w, args[2], args[3])
         made.append(plan)
         ctx.plan = plan
-        ctx.save_for_backward(x if w is not None else None, w, plan["slot_row"])
+        ctx.save_for_backward(x if w is not None else None, w)
         return rows
 
     @staticmethod
     @once_differentiable
     def backward(ctx, drows):
-        x, w, _ = ctx.saved_tensors
+        x, w = ctx.saved_tensors
         drows = drows.contiguous()
         if ctx.needs_input_grad[1]:
             dx, dw = K.unsort_rows(drows, ctx.plan, w, x=x)
