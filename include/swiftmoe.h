@@ -254,6 +254,21 @@ SMOE_API int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const i
                                int64_t rows_cap, int N, int K, void* dW, int out_dtype, void* workspace,
                                size_t workspace_bytes, smoe_stream_t stream);
 
+/* The three in one call: the gradients of smoe_grouped_linear's output (without its residual,
+ * whose gradient is dout) that are asked for -- dA [rows_cap, K], dW [G, N, K], dbias [G, N],
+ * each NULL or not -- from dout [rows_cap, N] and what the forward had (W in SMOE_W_NK, preact
+ * unless act is SMOE_ACT_NONE).  Rows of no group have no influence, and dA 0.  `grads` of the
+ * size query: SMOE_GRAD_* of the outputs asked for.                                      */
+#define SMOE_GRAD_A 1
+#define SMOE_GRAD_W 2
+#define SMOE_GRAD_BIAS 4
+SMOE_API size_t smoe_grouped_linear_bwd_workspace_size(int act, int grads, int dtype, int64_t rows_cap, int G, int N,
+                                                       int K);
+SMOE_API int smoe_grouped_linear_bwd(const void* dout, const void* A, const void* W, const void* preact, int act,
+                                     int dtype, const int32_t* offsets, int G, int64_t rows_cap, int N, int K, void* dA,
+                                     void* dW, void* dbias, int bias_dtype, void* workspace, size_t workspace_bytes,
+                                     smoe_stream_t stream);
+
 /* out[r, :] = [lo(w[r, :]) | hi(w[r, :]) | hi(w[r, :])] for `rows` fp32 rows of K (K % 4
  * == 0, 16-byte aligned): hi = the tf32 rounding (to nearest, ties away from zero), lo =
  * the exact remainder -- the weight layout the fp32 grouped GEMMs run on the tf32 tensor

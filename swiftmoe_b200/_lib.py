@@ -19,6 +19,7 @@ SMOE_F32_SPLITW = 16   # layer dtype: fp32 with routed expert weights split for 
 SMOE_EXPERT_LINEAR, SMOE_EXPERT_SWIGLU = 0, 1
 SMOE_EPI_STORE, SMOE_EPI_SWIGLU, SMOE_EPI_GATEUP = 0, 1, 3
 SMOE_W_NK, SMOE_W_KN = 0, 1
+SMOE_GRAD_A, SMOE_GRAD_W, SMOE_GRAD_BIAS = 1, 2, 4
 ACT_CODE = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}   # SMOE_ACT_*
 
 DTYPE_CODE = {torch.float32: SMOE_F32, torch.float16: SMOE_F16, torch.bfloat16: SMOE_BF16}
@@ -82,6 +83,9 @@ SIGNATURES = {
     "smoe_linear_act_bwd": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _i64, _i32, _vp, _sz, _vp]),
     "smoe_linear_wgrad_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
     "smoe_linear_wgrad": (_i32, [_vp, _vp, _i32, _vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp, _sz, _vp]),
+    "smoe_grouped_linear_bwd_workspace_size": (_sz, [_i32, _i32, _i32, _i64, _i32, _i32, _i32]),
+    "smoe_grouped_linear_bwd": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _i32,
+                                       _vp, _sz, _vp]),
     "smoe_grouped_gemm": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _vp]),
     "smoe_grouped_gemm_rows": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _vp]),
     "smoe_transpose_batched": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp]),

@@ -151,7 +151,7 @@ __device__ __forceinline__ void add_bias(const LinearEpi& lin, int64_t at, float
 // different row for every (slice s, group g) pair that has rows, since both only grow
 // along the rows.  bias_grad_reduce_kernel adds a group's partials in slice order, so no
 // result depends on the order in which blocks run.
-constexpr int kActCols = 256;
+constexpr int kActCols = 256, kActGroups = 1024;
 
 template <typename T, int ACT, bool BIAS>
 __global__ void __launch_bounds__(256, 4) linear_act_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ z,
@@ -159,20 +159,23 @@ __global__ void __launch_bounds__(256, 4) linear_act_bwd_kernel(const T* __restr
                                                              int G, int rows_cap, int N, int slice,
                                                              float* __restrict__ part) {
   __shared__ float s_sum[8][kActCols + 8];
+  __shared__ int s_off[kActGroups + 1];  // the walk over (mostly empty) groups waits for no load
+  for (int i = threadIdx.x; i <= G; i += 256) s_off[i] = offsets[i];
+  __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = blockIdx.x * kActCols + lane * 8;
   const bool live = col < N;
-  const int end_all = min(max(offsets[G], 0), rows_cap);
-  int row = max(blockIdx.y * slice, max(offsets[0], 0));
+  const int end_all = min(max(s_off[G], 0), rows_cap);
+  int row = max(blockIdx.y * slice, max(s_off[0], 0));
   const int row_end = min((int)blockIdx.y * slice + slice, end_all);
   if (row >= row_end) return;
   int lo = 0, hi = G - 1;  // last group whose start <= row
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (offsets[mid] <= row) lo = mid; else hi = mid - 1;
+    if (s_off[mid] <= row) lo = mid; else hi = mid - 1;
   }
   for (int g = lo; g < G && row < row_end; ++g) {
-    const int stop = min(offsets[g + 1], row_end);
+    const int stop = min(s_off[g + 1], row_end);
     if (stop <= row) continue;
     float sum[8];
 #pragma unroll

@@ -750,7 +750,9 @@ template <typename T, int VEC, int WPT>
 cudaError_t launch_sort_rows(const void* x, const int32_t* sr, const float* w, int T_, int k, int d,
                              const int32_t* row_token, const int32_t* offsets, int E, int64_t rows_cap, void* out,
                              const void* y, float* dw, cudaStream_t st) {
-  const unsigned grid = token_grid(T_, WPT, 64);
+  // enough blocks for the tokens and, should most rows be of no slot, for clearing them
+  const unsigned fill = (unsigned)std::min<int64_t>(cdiv(rows_cap * (d / VEC), 8 * rows::THREADS), device_sms());
+  const unsigned grid = std::max(token_grid(T_, WPT, 64), fill);
 #define SMOE_SORT(HW, DOT)                                                                                          \
   return launch_k(rows::sort_rows_kernel<T, VEC, WPT, HW, DOT>, grid, rows::THREADS, 0, st, (const T*)x, sr, w, T_, k, \
                   d, row_token, offsets, E, rows_cap, (T*)out, (const T*)y, dw)
@@ -1318,6 +1320,51 @@ int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const int32_t* o
   if (out_dtype == SMOE_F32) return launch_linear_wgrad<float>(ma, mb, dW, offsets, G, N, K, kr, idesc, ws, ks, st);
   return bf ? launch_linear_wgrad<__nv_bfloat16>(ma, mb, dW, offsets, G, N, K, kr, idesc, ws, ks, st)
             : launch_linear_wgrad<__half>(ma, mb, dW, offsets, G, N, K, kr, idesc, ws, ks, st);
+}
+
+namespace {
+// Slabs of smoe_grouped_linear_bwd's workspace: dz (for an activation), then one scratch that
+// the three steps use in turn.
+struct LinearBwd {
+  size_t dz, scratch;
+};
+LinearBwd linear_bwd_plan(int act, bool need_a, bool need_w, bool need_b, int dtype, int64_t rows_cap, int G, int N, int K) {
+  LinearBwd p;
+  p.dz = act != SMOE_ACT_NONE ? align_up((size_t)rows_cap * N * elt_size(dtype), 256) : 0;
+  p.scratch = need_b ? smoe_linear_act_bwd_workspace_size(rows_cap, N, G) : 0;
+  if (need_a) p.scratch = std::max(p.scratch, smoe_grouped_linear_workspace_size(rows_cap, K, N, G, SMOE_W_KN));
+  if (need_w) p.scratch = std::max(p.scratch, smoe_linear_wgrad_workspace_size(rows_cap, G, N, K));
+  return p;
+}
+}  // namespace
+
+size_t smoe_grouped_linear_bwd_workspace_size(int act, int grads, int dtype, int64_t rows_cap, int G, int N, int K) {
+  if (rows_cap < 1 || G < 1 || N < 1 || K < 1) return 0;
+  const LinearBwd p = linear_bwd_plan(act, grads & SMOE_GRAD_A, grads & SMOE_GRAD_W, grads & SMOE_GRAD_BIAS, dtype,
+                                      rows_cap, G, N, K);
+  return p.dz + p.scratch;
+}
+
+int smoe_grouped_linear_bwd(const void* dout, const void* A, const void* W, const void* preact, int act, int dtype,
+                            const int32_t* offsets, int G, int64_t rows_cap, int N, int K, void* dA, void* dW,
+                            void* dbias, int bias_dtype, void* workspace, size_t workspace_bytes,
+                            smoe_stream_t stream) {
+  if (G < 1 || N < 1 || K < 1 || rows_cap < 0) return SMOE_ERR_INVALID;
+  const LinearBwd p = linear_bwd_plan(act, dA, dW, dbias, dtype, rows_cap, G, N, K);
+  if (p.dz + p.scratch > 0 && (!workspace || workspace_bytes < p.dz + p.scratch)) return SMOE_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return SMOE_ERR_UNSUPPORTED;
+  void* dz = act != SMOE_ACT_NONE ? workspace : nullptr;
+  void* scratch = p.scratch > 0 ? static_cast<unsigned char*>(workspace) + p.dz : nullptr;
+  int rc = smoe_linear_act_bwd(dout, preact, act, dz, dbias, bias_dtype, dtype, offsets, G, rows_cap, N, scratch,
+                               p.scratch, stream);
+  if (rc) return rc;
+  const void* g = dz ? dz : dout;
+  if (dA) {
+    rc = smoe_grouped_linear(g, W, SMOE_W_KN, nullptr, dtype, SMOE_ACT_NONE, nullptr, nullptr, 1, dA, dtype, offsets, G,
+                             rows_cap, K, N, scratch, p.scratch, stream);
+    if (rc) return rc;
+  }
+  return dW ? smoe_linear_wgrad(g, A, dtype, offsets, G, rows_cap, N, K, dW, dtype, scratch, p.scratch, stream) : SMOE_OK;
 }
 
 int smoe_grouped_gemm(const void* A, const void* B, const void* B3, void* C, int dtype, int out_dtype, int epilogue,

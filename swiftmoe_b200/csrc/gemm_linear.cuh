@@ -273,7 +273,7 @@ __device__ __forceinline__ void fill_other_rows(const LinearEpi& lin, T* __restr
 // 4096 x 4096 weights, whose bytes take 5.)  ks is the cheapest by a count of k-blocks per
 // CTA: whole waves of units, each with its share of the K blocks, about 3 blocks' time to
 // fill the ring and drain the tile, and for its partial tile's way out and back 8 blocks'
-// time per 128 rows; the second launch counts 6.  Both launches compute it from the same
+// time per 128 rows; the second launch counts 16.  Both launches compute it from the same
 // numbers.  rows: rows of a slot.
 // (32-bit divisions: one thread of every block works this out before the block can start.)
 __host__ __device__ inline int split_units(uint32_t tiles, uint32_t kb, uint32_t rows, uint32_t ctas, uint32_t slots) {
@@ -282,7 +282,7 @@ __host__ __device__ inline int split_units(uint32_t tiles, uint32_t kb, uint32_t
   for (uint32_t ks = 1; ks <= MAX_SPLIT; ++ks) {
     if (ks > 1 && (tiles > slots / ks || kb < 4 * ks)) break;
     const uint32_t waves = (tiles * ks + ctas - 1) / ctas, blocks = (kb + ks - 1) / ks + 3;
-    const uint64_t cost = (uint64_t)waves * (blocks * 16 + (ks > 1 ? rows : 0)) + (ks > 1 ? 6 * 16 : 0);
+    const uint64_t cost = (uint64_t)waves * (blocks * 16 + (ks > 1 ? rows : 0)) + (ks > 1 ? 16 * 16 : 0);
     if (cost < best_cost) {
       best_cost = cost;
       best = (int)ks;

@@ -177,7 +177,8 @@ __global__ void __launch_bounds__(THREADS) sort_rows_kernel(const T* __restrict_
       }
     };
     if (mask != 0) {
-      constexpr int U = WPT == 1 ? 8 : 2;  // a row of 4096 bf16 is 2 x 8 x 32 pieces, or 2 x 8 warps
+      // a row of 4096 bf16 is 2 x 8 x 32 pieces, or 2 x 8 warps; single elements, more of them
+      constexpr int U = (WPT == 1 ? 8 : 2) * (sizeof(T) * VEC < 16 ? 2 : 1);
       int c = part * 32;
       for (; c + (U - 1) * STEP + 32 <= nv; c += U * STEP) step(Int<U>(), Int<1>(), c + lane);
       for (; c < nv; c += STEP) step(Int<1>(), Int<0>(), c + lane);
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(THREADS) unsort_rows_kernel(const T* __restric
                                                               T* __restrict__ out, const T* __restrict__ x,
                                                               float* __restrict__ dw) {
   pdl_wait_and_release();
-  constexpr int U = DOT && WPT == 1 ? 4 : 2, TPB = WARPS / WPT;
+  constexpr int U = (DOT && WPT == 1 ? 4 : 2) * (sizeof(T) * VEC < 16 ? 4 : 1), TPB = WARPS / WPT;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = warp % WPT;
   const int nv = d / VEC;

@@ -24,7 +24,6 @@ from typing import Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib as L
 from . import kernels as K
 
 
@@ -91,11 +90,8 @@ class _GroupedLinear(torch.autograd.Function):
         dout = dout.contiguous()
         da = dw = db = None
         if need_a or need_w or need_b:
-            dz, db = K.linear_act_bwd(dout, offsets, ctx.activation, z, ctx.bias_dtype if need_b else None)
-            if need_a:
-                da = K.grouped_linear(dz, weight, offsets, w_layout=L.SMOE_W_KN)
-            if need_w:
-                dw = K.linear_wgrad(dz, a, offsets)
+            da, dw, db = K.grouped_linear_bwd(dout, a, weight, offsets, ctx.activation, z, need_a=need_a, need_w=need_w,
+                                              bias_dtype=ctx.bias_dtype if need_b else None)
         return da, dw, db, dout if need_res else None, None, None
 
 

@@ -79,6 +79,20 @@ def test_linear_refusals(lib):
         assert wg(**bad) == -4, bad
 
 
+def test_linear_backward_refusals(lib):
+    bwd = lambda **a: lib.smoe_grouped_linear_bwd(*{**dict(dout=P, A=P, W=P, z=P, act=2, dt=BF, off=P, G=2, R=30, N=16, K=16,  # noqa: E731
+                                                           dA=P, dW=P, db=P, bdt=BF, ws=P, wsb=1 << 26, st=None), **a}.values())
+    for bad in (dict(G=0), dict(N=0), dict(K=0), dict(R=-1), dict(act=9), dict(dout=None), dict(z=None), dict(off=None)):
+        assert bwd(**bad) == -1, bad
+    for bad in (dict(dt=F32), dict(N=12), dict(bdt=1), dict(ws=P + 8), dict(dout=P + 2)):
+        assert bwd(**bad) == -4, bad
+    assert bwd(ws=None) == -5 and bwd(wsb=100) == -5
+    size = lib.smoe_grouped_linear_bwd_workspace_size
+    assert size(0, 7, BF, 0, 2, 16, 16) == 0 and size(0, 1, BF, 20000, 2, 16, 128) == 0
+    assert size(2, 0, BF, 100, 2, 16, 16) == 3328                         # dz alone, 256-byte slabs
+    assert size(2, 4, BF, 100, 2, 16, 16) > 3328
+
+
 def test_workspace_sizes(lib):
     # partial tiles only where a launch can have few of them
     assert lib.smoe_grouped_linear_workspace_size(2, 4096, 4096, 8, L.SMOE_W_NK) == 0       # decode kernel
