@@ -157,7 +157,7 @@ SMOE_API int smoe_combine(const void* y, int dtype, const int32_t* slot_row, con
  * The two directions of the routed rows as operators of their own, with the gate weights
  * and what their gradients need.  slot_row, row_token and expert_offsets are those of a
  * dispatch plan; rows_cap is the row count of `rows` / `y`; w [T,k] fp32 or NULL (all 1);
- * k <= 32 (else SMOE_ERR_UNSUPPORTED).  Sums are fp32 in slot order, rounded once.
+ * k <= 32, d <= 2^30 and rows_cap < 2^31 - 65535 (else SMOE_ERR_UNSUPPORTED).  Sums are fp32 in slot order, rounded once.
  *
  * smoe_sort_rows: rows[slot_row[t,j],:] = w[t,j] * x[t,:]; every other row of the
  * rows_cap rows becomes zero: those from expert_offsets[E] on and, when row_token is
@@ -228,7 +228,8 @@ SMOE_API int smoe_grouped_gemm_rows(const void* A, const void* B, const void* B3
  * Rows of no group -- before offsets[0] or from offsets[G] on -- are left as they were, or,
  * with fill != 0, become residual (zeros without one).  offsets are non-decreasing and live
  * in device memory; they are clamped into [0, rows_cap].  bf16 / fp16, N and K multiples of
- * 8, 16-byte aligned pointers, G <= 1024.  At most 2 rows stream the weights on the SIMT
+ * 8 up to 2^30, 16-byte aligned pointers, G <= 1024, rows_cap < 2^31 - 65535; C must not
+ * overlap A.  At most 2 rows stream the weights on the SIMT
  * pipes (SMOE_W_NK), everything else runs on tcgen05 tensor cores; launches of few tiles
  * split K over otherwise idle SMs through the workspace (its size may be 0).
  * Replaces: nn.Linear experts with a bias around models/baseline_moe.py:151-162 (the
@@ -248,7 +249,8 @@ SMOE_API int smoe_linear_act_bwd(const void* dout, const void* preact, int act, 
                                  size_t workspace_bytes, smoe_stream_t stream);
 /* Weight gradient dW[g] = dz_g^T A_g, [G, N, K] in dtype or fp32 (out_dtype), dz
  * [rows_cap, N], A [rows_cap, K].  Groups may start at any row; a group without rows gets
- * zeros.  Few tiles are split along the rows through the workspace (its size may be 0).  The input gradient is smoe_grouped_linear(dz, W, SMOE_W_KN).                  */
+ * zeros.  Few tiles are split along the rows through the workspace (its size may be 0).
+ * The input gradient is smoe_grouped_linear(dz, W, SMOE_W_KN).                          */
 SMOE_API size_t smoe_linear_wgrad_workspace_size(int64_t rows_cap, int G, int N, int K);
 SMOE_API int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const int32_t* offsets, int G,
                                int64_t rows_cap, int N, int K, void* dW, int out_dtype, void* workspace,

@@ -595,6 +595,11 @@ int grouped_gemm_impl(const void* A, const void* B, const void* B3, void* C, int
                             : launch_tc<SMOE_EPI_STORE, __half>(ma, mb, mb3, C, N, row_ptrs, offsets, ends, G, rows_cap, N, K, idesc, st);
 }
 
+// Largest sizes of the routed-row operators: the kernels step through rows and columns with
+// 32-bit counters, up to a slice (rows) or a few thousand columns past the end.
+constexpr int64_t kMaxRows = INT32_MAX - 65535;
+constexpr int kMaxCols = 1 << 30;
+
 // ------------------------------------------------------------------ grouped linear layers
 // 3-D map over [G, K, N] weights read along N: box = 64 columns (N) x 64 rows (K) x 1 group,
 // an MN-major operand tile.
@@ -707,10 +712,12 @@ int launch_linear_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, void* C, c
 }
 
 // Rows of one block (and of one partial sum of the bias gradient): a multiple of its eight
-// warps that makes about eight blocks per SM, at least 16, at most 512.
+// warps that makes about eight blocks per SM, at least 16, at most 512 -- or, beyond 33.5
+// million rows, what keeps the slices within a grid's 65535 blocks in y.
 int act_bwd_slice(int64_t rows_cap, int N) {
   const int64_t slices = std::max<int64_t>(1, (int64_t)device_sms() * 8 / cdiv(N, kActCols));
-  return (int)std::min<int64_t>(512, std::max<int64_t>(16, align_up((size_t)cdiv(rows_cap, slices), 8)));
+  const int64_t slice = std::min<int64_t>(512, std::max<int64_t>(16, cdiv(rows_cap, slices)));
+  return (int)align_up((size_t)std::max<int64_t>(slice, cdiv(rows_cap, 65535)), 8);
 }
 
 template <typename T, bool BIAS>
@@ -1156,7 +1163,7 @@ int smoe_sort_rows(const void* x, int dtype, const int32_t* slot_row, const floa
                    const void* y, float* dw, smoe_stream_t stream) {
   const int es = elt_size(dtype);
   if (es == 0 || T < 0 || k < 1 || d < 1 || E < 1 || rows_cap < 0) return SMOE_ERR_INVALID;
-  if (k > rows::MAX_K || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (k > rows::MAX_K || d > kMaxCols || rows_cap > kMaxRows) return SMOE_ERR_UNSUPPORTED;
   if (T == 0 && rows_cap == 0) return SMOE_OK;
   if (!expert_offsets || (rows_cap > 0 && !rows) || (T > 0 && (!x || !slot_row)) || (dw && (!w || (rows_cap > 0 && !y))))
     return SMOE_ERR_INVALID;
@@ -1176,7 +1183,7 @@ int smoe_sort_tokens(const void* x, int dtype, const int32_t* idx, const float* 
                      smoe_stream_t stream) {
   // everything the second call refuses, before the first one launches
   if (elt_size(dtype) == 0 || d < 1 || (T > 0 && !x) || (rows_cap > 0 && !rows)) return SMOE_ERR_INVALID;
-  if (k > rows::MAX_K || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (k > rows::MAX_K || d > kMaxCols || rows_cap > kMaxRows) return SMOE_ERR_UNSUPPORTED;
   // each launch is scheduled while its short predecessor finishes
   const PdlScope pdl(true);
   const int rc = smoe_dispatch_plan(idx, T, k, E, capacity, row_align, expert_counts, expert_offsets, slot_row, row_token,
@@ -1191,7 +1198,7 @@ int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const fl
                      smoe_stream_t stream) {
   const int es = elt_size(dtype);
   if (es == 0 || T < 0 || k < 1 || d < 1 || rows_cap < 0) return SMOE_ERR_INVALID;
-  if (k > rows::MAX_K || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (k > rows::MAX_K || d > kMaxCols || rows_cap > kMaxRows) return SMOE_ERR_UNSUPPORTED;
   if (T == 0) return SMOE_OK;
   if (!slot_row || !out || (rows_cap > 0 && !y) || (dw && (!w || !x))) return SMOE_ERR_INVALID;
   const int vec = row_vec(es, d, {y, out, residual, dw ? x : nullptr}), wpt = token_warps(T, d / vec);
@@ -1219,7 +1226,8 @@ int smoe_grouped_linear(const void* A, const void* W, int w_layout, const void* 
   if (w_layout != SMOE_W_NK && w_layout != SMOE_W_KN) return SMOE_ERR_INVALID;
   if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_UNSUPPORTED;
   if (bias && bias_dtype != dtype && bias_dtype != SMOE_F32) return SMOE_ERR_UNSUPPORTED;
-  if (N % 8 != 0 || K % 8 != 0 || G > tc::MAX_GROUPS || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (N % 8 != 0 || K % 8 != 0 || std::max(N, K) > kMaxCols) return SMOE_ERR_UNSUPPORTED;
+  if (G > tc::MAX_GROUPS || rows_cap > kMaxRows) return SMOE_ERR_UNSUPPORTED;
   if (rows_cap == 0) return SMOE_OK;
   if (!A || !W || !C || !offsets) return SMOE_ERR_INVALID;
   for (const void* p : {A, W, bias, residual, (const void*)preact, (const void*)C, (const void*)workspace})
@@ -1254,7 +1262,7 @@ int smoe_linear_act_bwd(const void* dout, const void* preact, int act, void* dz,
   if (G < 1 || N < 1 || rows_cap < 0 || act < SMOE_ACT_NONE || act > SMOE_ACT_SILU) return SMOE_ERR_INVALID;
   if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_UNSUPPORTED;
   if (dbias && bias_dtype != dtype && bias_dtype != SMOE_F32) return SMOE_ERR_UNSUPPORTED;
-  if (N % 8 != 0 || G > tc::MAX_GROUPS || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (N % 8 != 0 || N > kMaxCols || G > tc::MAX_GROUPS || rows_cap > kMaxRows) return SMOE_ERR_UNSUPPORTED;
   cudaStream_t st = (cudaStream_t)stream;
   if (rows_cap == 0) {
     if (dbias) SMOE_CK(cudaMemsetAsync(dbias, 0, (size_t)G * N * elt_size(bias_dtype), st));
@@ -1298,7 +1306,8 @@ int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const int32_t* o
   if (G < 1 || N < 1 || K < 1 || rows_cap < 0 || !offsets || !dW) return SMOE_ERR_INVALID;
   if (dtype != SMOE_BF16 && dtype != SMOE_F16) return SMOE_ERR_UNSUPPORTED;
   if (out_dtype != dtype && out_dtype != SMOE_F32) return SMOE_ERR_UNSUPPORTED;
-  if (N % 8 != 0 || K % 8 != 0 || G > tc::MAX_GROUPS || rows_cap > INT32_MAX) return SMOE_ERR_UNSUPPORTED;
+  if (N % 8 != 0 || K % 8 != 0 || std::max(N, K) > kMaxCols) return SMOE_ERR_UNSUPPORTED;
+  if (G > tc::MAX_GROUPS || rows_cap > kMaxRows) return SMOE_ERR_UNSUPPORTED;
   cudaStream_t st = (cudaStream_t)stream;
   if (rows_cap == 0) {
     SMOE_CK(cudaMemsetAsync(dW, 0, (size_t)G * N * K * elt_size(out_dtype), st));

@@ -43,6 +43,12 @@ def _device_of(first: torch.Tensor, *ts) -> torch.device:
 
 
 _HERE = nullcontext()
+_MAX_INT, _MAX_COLS = 2**31 - 1, 2**30   # what the library's int arguments hold; its columns
+
+
+def _columns(*n: int):
+    if max(n) > _MAX_COLS:
+        raise L.SwiftMoEError(f"more than 2^30 columns: {max(n)}")
 
 
 def _on(device):
@@ -145,6 +151,8 @@ def _plan_args(plan: dict, rows: int, w: Optional[torch.Tensor]):
     slot_row, offsets, T, k = plan["slot_row"], plan["offsets"], plan["T"], plan["k"]
     if slot_row.dtype != torch.int32 or offsets.dtype != torch.int32 or slot_row.numel() != T * k:
         raise L.SwiftMoEError("not a dispatch plan: slot_row must be int32 [T*k], offsets int32")
+    if T * k > _MAX_INT:
+        raise L.SwiftMoEError("a plan has at most 2^31 - 1 slots")
     if rows < plan["rows_cap"]:
         raise L.SwiftMoEError(f"the plan has up to {plan['rows_cap']} rows, the tensor only {rows}")
     if w is not None and (w.dtype != torch.float32 or w.shape != (T, k)):
@@ -169,6 +177,7 @@ def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, 
     if row_token is not None and (row_token.dtype != torch.int32 or row_token.numel() < plan["rows_cap"]):
         raise L.SwiftMoEError("not a dispatch plan: row_token must be int32 [rows_cap]")
     d = x.shape[1]
+    _columns(d)
     if y is not None and (w is None or y.dtype != x.dtype or y.shape != (rows_cap, d)):
         raise L.SwiftMoEError("y needs weights, x's dtype and shape [rows_cap, d]")
     dt = L.dtype_code(x.dtype)
@@ -193,6 +202,9 @@ def sort_tokens(x: torch.Tensor, idx: torch.Tensor, num_experts: int, w: Optiona
     if w is not None and (w.dtype != torch.float32 or w.shape != idx.shape):
         raise L.SwiftMoEError(f"weights must be float32 [{T}, {k}], got {w.dtype} {tuple(w.shape)}")
     dt, d, E, lib, i32 = L.dtype_code(x.dtype), x.shape[1], num_experts, L.load(), torch.int32
+    if T * k > _MAX_INT:
+        raise L.SwiftMoEError("a plan has at most 2^31 - 1 slots")
+    _columns(d)
     rows_cap = lib.smoe_plan_rows_cap(T, k, E, capacity, row_align)
     need = lib.smoe_plan_workspace_size(T, k, E)
     if E < 1:
@@ -222,6 +234,7 @@ def unsort_rows(y: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, r
     if y.dim() != 2:
         raise L.SwiftMoEError(f"rows must be [rows, d], got {tuple(y.shape)}")
     rows_cap, d = y.shape
+    _columns(d)
     slot_row, _, T, k = _plan_args(plan, rows_cap, w)
     dev = _device_of(y, slot_row, w, residual, x)
     for name, t in (("residual", residual), ("x", x)):
@@ -273,6 +286,7 @@ def grouped_linear(A: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, bias
     G, N, K2 = W.shape if w_layout == L.SMOE_W_NK else (W.shape[0], W.shape[2], W.shape[1])
     if K2 != Kd:
         raise L.SwiftMoEError("K mismatch")
+    _columns(N, Kd)
     _group_offsets(offsets, G)
     if bias is not None and (bias.shape != (G, N) or bias.dtype not in (A.dtype, torch.float32)):
         raise L.SwiftMoEError(f"bias must be {A.dtype} or float32 [{G}, {N}], got {bias.dtype} {tuple(bias.shape)}")
@@ -301,6 +315,7 @@ def linear_act_bwd(dout: torch.Tensor, offsets: torch.Tensor, activation: str, p
     act, dt = _act_code(activation), _linear_dtype(dout)
     rows_cap, N = dout.shape
     G = offsets.numel() - 1
+    _columns(N)
     _group_offsets(offsets, G)
     if act and (preact is None or preact.dtype != dout.dtype or preact.shape != dout.shape):
         raise L.SwiftMoEError("preact must have dout's dtype and shape")
@@ -327,6 +342,7 @@ def linear_wgrad(dz: torch.Tensor, A: torch.Tensor, offsets: torch.Tensor,
         raise L.SwiftMoEError("dz [rows, N] and A [rows, K] must have the same rows and dtype")
     rows_cap, N = dz.shape
     Kd, G = A.shape[1], offsets.numel() - 1
+    _columns(N, Kd)
     _group_offsets(offsets, G)
     od = A.dtype if out_dtype is None else out_dtype
     dW = torch.empty((G, N, Kd), dtype=od, device=dev)
@@ -354,6 +370,7 @@ def grouped_linear_bwd(dout: torch.Tensor, A: torch.Tensor, W: torch.Tensor, off
     G, N, K2 = W.shape
     if K2 != Kd or dout.shape != (rows_cap, N):
         raise L.SwiftMoEError("dout must be [rows, N], A [rows, K]")
+    _columns(N, Kd)
     _group_offsets(offsets, G)
     if act and (preact is None or preact.dtype != A.dtype or preact.shape != dout.shape):
         raise L.SwiftMoEError("preact must have dout's dtype and shape")

@@ -105,3 +105,22 @@ def test_workspace_sizes(lib):
     # bias partials: a row per slice (16 to 512 rows) and one per group
     assert lib.smoe_linear_act_bwd_workspace_size(64, 8, 4) == (4 + 4) * 8 * 4
     assert lib.smoe_linear_act_bwd_workspace_size(1 << 20, 8, 4) == ((1 << 20) // 512 + 4) * 8 * 4
+
+
+def test_largest_sizes(lib):
+    # the last sizes the 32-bit counters of the kernels can pass are refused before any launch
+    most, cols = (1 << 31) - 1 - 65535, (1 << 30) + 8
+    assert lib.smoe_sort_rows(P, BF, P, None, 4, 2, 8, None, P, 2, most + 1, P, None, None, None) == -4
+    assert lib.smoe_sort_rows(P, BF, P, None, 4, 2, cols, None, P, 2, 8, P, None, None, None) == -4
+    assert lib.smoe_unsort_rows(P, BF, P, None, 4, 2, 8, most + 1, None, P, None, None, None) == -4
+    assert lib.smoe_unsort_rows(P, BF, P, None, 4, 2, cols, 8, None, P, None, None, None) == -4
+    for rows, n, k in ((most + 1, 8, 8), (8, cols, 8), (8, 8, cols)):
+        assert lib.smoe_grouped_linear(P, P, 0, None, BF, 0, None, None, 1, P, BF, P, 2, rows, n, k, None, 0, None) == -4
+        assert lib.smoe_linear_wgrad(P, P, BF, P, 2, rows, n, k, P, BF, None, 0, None) == -4
+    for rows, n in ((most + 1, 8), (8, cols)):
+        assert lib.smoe_linear_act_bwd(P, P, 2, P, None, BF, BF, P, 2, rows, n, None, 0, None) == -4
+    # the bias gradient's slices of rows are a grid's y blocks
+    for rows in (512 * 65535, 512 * 65535 + 1, 1 << 26, most):
+        for n in (8, 64, 4096):
+            slices = lib.smoe_linear_act_bwd_workspace_size(rows, n, 4) // (n * 4) - 4
+            assert 0 < slices <= 65535, (rows, n, slices)
