@@ -60,7 +60,7 @@ template <int ACT> __device__ __forceinline__ float act_f(float z) {
 }
 
 template <int ACT> __device__ __forceinline__ float act_slope(float z) {
-  if constexpr (ACT == SMOE_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if constexpr (ACT == SMOE_ACT_RELU) return z <= 0.0f ? 0.0f : 1.0f;  // NaN: the gradient passes
   if constexpr (ACT == SMOE_ACT_GELU) {  // Phi(z) + z phi(z)
     float e;
     const float phi = normal_cdf(z, e);

@@ -277,7 +277,8 @@ def grouped_linear(A: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, bias
     """C[r] = act(A[r] W_g^T + bias[g]) + residual[r] for the rows r of group g, [offsets[g],
     offsets[g+1]); W [G, N, K] (``L.SMOE_W_KN``: [G, K, N], C = A W_g), bias [G, N] in A's dtype
     or fp32.  Rows of no group become the residual alone (zeros without one); given ``out``,
-    its rows of no group stay as they were.  ``preact`` [rows, N] receives A W_g^T + bias[g]."""
+    its rows of no group stay as they were (it may be the residual, but must not overlap A).
+    ``preact`` [rows, N] receives A W_g^T + bias[g]."""
     dev = _device_of(A, W, offsets, bias, residual, preact, out)
     act, dt = _act_code(activation), _linear_dtype(A)
     if A.dim() != 2 or W.dim() != 3 or W.dtype != A.dtype:

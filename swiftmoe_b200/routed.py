@@ -88,6 +88,8 @@ class _GroupedLinear(torch.autograd.Function):
         a, weight, offsets, z = ctx.saved_tensors
         need_a, need_w, need_b, need_res = ctx.needs_input_grad[:4]
         dout = dout.contiguous()
+        if dout.data_ptr() % 16:   # a piece of a larger gradient: the kernels load 16 bytes at a time
+            dout = dout.clone()
         da = dw = db = None
         if need_a or need_w or need_b:
             da, dw, db = K.grouped_linear_bwd(dout, a, weight, offsets, ctx.activation, z, need_a=need_a, need_w=need_w,

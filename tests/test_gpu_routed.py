@@ -430,6 +430,37 @@ def test_grouped_linear_gradient_against_differences(S, act):
         assert abs(float(want - got)) <= 6 * math.sqrt(float(var)) + float(curve)
 
 
+def test_gradient_that_starts_off_a_16_byte_boundary(S):
+    c = group_case([70, 0, 33], 64, 72, torch.bfloat16, 1, 1, 2)
+    leaves = [c[n].clone().requires_grad_() for n in "awbr"]
+    want = torch.autograd.grad(S.grouped_linear(leaves[0], leaves[1], c["off"], leaves[2], "gelu", leaves[3]), leaves, c["dout"])
+    buf = torch.empty(c["dout"].numel() + 1, dtype=torch.bfloat16, device="cuda")
+    dout = buf[1:].view(c["dout"].shape).copy_(c["dout"])
+    got = torch.autograd.grad(S.grouped_linear(leaves[0], leaves[1], c["off"], leaves[2], "gelu", leaves[3]), leaves, dout)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("sizes", [[1, 0, 1], [70, 0, 33], [300, 500, 200]])
+def test_residual_in_place(S, K, sizes):
+    """out may be the residual: rows of two decode kernels, a split and a whole launch."""
+    c = group_case(sizes, 1024, 72, torch.bfloat16, 1, 1 if sum(sizes) > 2 else 0, 0)
+    want = S.grouped_linear(c["a"], c["w"], c["off"], c["b"], "silu", c["r"])
+    out = c["r"].clone()
+    assert K.grouped_linear(c["a"], c["w"], c["off"], c["b"], "silu", out, out=out) is out
+    assert torch.equal(out, want)
+
+
+def test_relu_passes_the_gradient_at_nan(S):
+    c = group_case([40], 64, 24, torch.bfloat16, 3, 0, 0, residual=False)
+    a, b, ones = c["a"].clone(), c["b"].clone().requires_grad_(), torch.ones_like(c["dout"])
+    rest = ones.clone()
+    rest[7] = 0
+    others, = torch.autograd.grad(S.grouped_linear(a, c["w"], c["off"], b, "relu"), [b], rest)
+    a[7] = float("nan")
+    every, = torch.autograd.grad(S.grouped_linear(a, c["w"], c["off"], b, "relu"), [b], ones)
+    assert torch.equal(every, others + 1)   # counts of rows, exact in bf16
+
+
 def test_infinities_and_nan_stay_in_their_rows(S):
     """A NaN or infinity in a group's rows reaches that row's outputs and that group's weight
     gradient only, whatever tile it shares."""
