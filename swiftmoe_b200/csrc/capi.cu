@@ -348,8 +348,9 @@ int launch_tc_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorM
   return SMOE_OK;
 }
 
-// Raster band (m-tiles) of the weight-gradient GEMMs.  8 x 14336 x 4096 bf16 weights from 16384
-// rows, at the power cap: n fastest 1.83 ms, bands of 8 / 16 / 32 m-tiles 1.52 / 1.52 / 1.50 ms.
+// Raster band (m-tiles) of the weight-gradient GEMMs.  4 x 4096 x 7168 bf16 weights from 8192
+// rows: 114 M sectors read from L2 and 382 us against 151 M and 393 with n fastest; bands of
+// 8 / 16 / 32 m-tiles take 1.52 / 1.52 / 1.50 ms for 8 x 14336 x 4096 from 16384 rows.
 constexpr int kWgradBand = 32;
 
 template <bool MN>

@@ -9,9 +9,9 @@
 //     warps about 19k cycles, more than the products of a tile up to K = 2400;
 //   * weights in either layout: [N, K] K-major, or [K, N] as an MN-major operand (the input
 //     gradient reads the weights as they are, no transposed copy);
-//   * two producer warps: one thread gets a box out about every 60 cycles plus its transfer,
-//     and the four to six boxes of an MN-major stage then take longer than the 512 cycles
-//     of its MMAs (input gradient of 16384 x 14336 x 4096: 1.70 -> 1.42 ms);
+//   * two producer warps, which share the four to six boxes of an MN-major stage (a stage's
+//     MMAs take 512 cycles; input gradient of 16384 x 14336 x 4096: 1.39 to 1.50 ms with one
+//     warp, 1.38 to 1.42 with two, 1.70 with one that also leaves out boxes past N);
 //   * launches of few tiles cut along K, the partial tiles summed by a second launch over the
 //     whole GPU (split_units below);
 //   * weight-gradient groups that start at any row, 16-bit gradients.
@@ -113,8 +113,8 @@ __device__ __forceinline__ uint32_t idesc_cols(uint32_t idesc, int cols) {
 // Eight 16-byte pieces per lane -- 128 bytes of the lane's row of a warp's 32 accumulator
 // rows -- to global memory by way of the warp's 2 KB stage, 16 rows at a time, so that a
 // warp store writes whole 128-byte lines of four rows instead of 16 bytes of 32 (the
-// load/store unit takes one step per row; 64-byte pieces of eight rows wrote gradients of
-// 0.94 GB at 4.4 TB/s against 5.9).  The pieces are XOR-swizzled by row: conflict-free both
+// load/store unit takes one step per row; a weight gradient of 0.94 GB from one row per
+// group: 214 us with 64-byte pieces of eight rows, 171 with these).  The pieces are XOR-swizzled by row: conflict-free both
 // ways.  Row rr goes to p + rr * pitch bytes; rows from nrows on and bytes from `width` on
 // are left out.
 __device__ __forceinline__ void store_rows128(const uint4 (&u)[8], unsigned char* p, int64_t pitch, int nrows,
@@ -270,7 +270,7 @@ __device__ __forceinline__ void fill_other_rows(const LinearEpi& lin, T* __restr
 // launch adds a tile's slices in order (so no result depends on which unit ends first) and
 // applies the epilogue, spread over the whole GPU.  (With the last unit of a tile adding
 // them up itself, its one CTA took longer than the products: 35 us for 64 rows against
-// 4096 x 4096 weights, whose bytes take 5.)  ks is the cheapest by a count of k-blocks per
+// 4096 x 4096 weights, now 18; the bytes take 5.)  ks is the cheapest by a count of k-blocks per
 // CTA: whole waves of units, each with its share of the K blocks, about 3 blocks' time to
 // fill the ring and drain the tile, and for its partial tile's way out and back 8 blocks'
 // time per 128 rows; the second launch counts 16.  Both launches compute it from the same
