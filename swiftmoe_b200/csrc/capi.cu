@@ -348,11 +348,6 @@ int launch_tc_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorM
   return SMOE_OK;
 }
 
-// Raster band (m-tiles) of the weight-gradient GEMMs.  4 x 4096 x 7168 bf16 weights from 8192
-// rows: 114 M sectors read from L2 and 382 us against 151 M and 393 with n fastest; bands of
-// 8 / 16 / 32 m-tiles take 1.52 / 1.52 / 1.50 ms for 8 x 14336 x 4096 from 16384 rows.
-constexpr int kWgradBand = 32;
-
 template <bool MN>
 int launch_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, float* C, const int32_t* koff, int G, int M, int N,
                  uint32_t idesc, cudaStream_t st) {
@@ -361,7 +356,9 @@ int launch_wgrad(const CUtensorMap& ma, const CUtensorMap& mb, float* C, const i
   SMOE_CK(ensure_smem(kern, tc::SMEM_BYTES_ROWS, &done));
   const int64_t tiles = (int64_t)G * cdiv(M, tc::BM) * cdiv(N, tc::BN);
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sms()));
-  kern<<<grid, tc::THREADS, tc::SMEM_BYTES_ROWS, st>>>(ma, mb, C, koff, G, M, N, idesc, kWgradBand);
+  // keep the smaller operand (per group: N rows of B against M rows of A) in L2: bands of one
+  // m-tile run its n-tiles back to back, one band of all m-tiles the other way round
+  kern<<<grid, tc::THREADS, tc::SMEM_BYTES_ROWS, st>>>(ma, mb, C, koff, G, M, N, idesc, N <= M ? 1 : (int)cdiv(M, tc::BM));
   SMOE_CK(cudaGetLastError());
   return SMOE_OK;
 }
@@ -685,6 +682,11 @@ int linear_gemm_t(const void* A, const void* B, void* C, const int32_t* offsets,
   }
   return SMOE_OK;
 }
+
+// Raster band (m-tiles) of the weight gradients.  16384 rows, 8 groups, bands of 1 (n fastest) /
+// 8 / 32 / 64 m-tiles: 1.53 / 1.54 / 1.51 / 1.53 ms for 14336 x 4096 weights, 1.75-1.85 / 1.71-1.76
+// / 1.68-1.71 / 1.67-1.72 for 4096 x 14336; 2.0 / 1.8 / 1.7-1.8 / 1.8 for 8192 rows, 28672 x 4096.
+constexpr int kWgradBand = 32;
 
 // K slices of a weight gradient's tiles, for evenly filled groups.
 int wgrad_slices(int64_t rows_cap, int G, int N, int K) {
