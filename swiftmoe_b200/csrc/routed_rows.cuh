@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(THREADS) unsort_rows_kernel(const T* __restric
                                                               T* __restrict__ out, const T* __restrict__ x,
                                                               float* __restrict__ dw) {
   pdl_wait_and_release();
-  constexpr int U = (DOT && WPT == 1 ? 4 : 2) * (sizeof(T) * VEC < 16 ? 4 : 1), TPB = WARPS / WPT;
+  constexpr int BYTES = sizeof(T) * VEC;
+  constexpr int U = (DOT && WPT == 1 ? 4 : 2) * (BYTES == 16 ? 1 : BYTES == 8 ? 2 : 4), TPB = WARPS / WPT;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = warp % WPT;
   const int nv = d / VEC;

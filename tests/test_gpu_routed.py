@@ -73,6 +73,7 @@ ROWS = [  # T, d, E, k, capacity, align, pad
     (1, 8, 1, 1, 0, 1, 0),
     (5, 24, 4, 3, 0, 8, 2),        # 16-bit rows of 48 bytes
     (37, 1030, 13, 3, 7, 1, 5),    # even, not a multiple of 8; capacity
+    (2000, 1034, 5, 2, 0, 8, 30),  # the same, one warp per token, several full steps
     (64, 129, 8, 8, 0, 64, 0),     # odd length, every expert of every token
     (33, 72, 40, 32, 3, 4, 9),     # k = 32
     (700, 264, 6, 2, 100, 1, 100),  # one warp per token
