@@ -21,6 +21,14 @@ __device__ __forceinline__ float rcp_fast(float v) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
+// v within [-lim, lim], NaN kept.
+__device__ __forceinline__ float clamp_nan(float v, float lim) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(lim));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(-lim));
+  return r;
+}
+
 // sigmoid(v) = 1 / (1 + e^-v): e^-v may be infinite, the quotient is then 0.
 __device__ __forceinline__ float sigmoid_f(float v) { return rcp_fast(1.0f + exp2_fast(-kLog2e * v)); }
 
@@ -59,22 +67,24 @@ template <int ACT> __device__ __forceinline__ float act_f(float z) {
   return z;
 }
 
+// z may be infinite where the forward was finite: it is kept rounded to the layer's type,
+// and fp16 ends at 65504.  The slopes are 0 or 1 to fp32 long before the clamps' limits
+// (GELU's beyond 15, SiLU's beyond 105), which keep 0 * infinity out of them.
 template <int ACT> __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == SMOE_ACT_RELU) return z <= 0.0f ? 0.0f : 1.0f;  // NaN: the gradient passes
   if constexpr (ACT == SMOE_ACT_GELU) {  // Phi(z) + z phi(z)
+    z = clamp_nan(z, 30.0f);
     float e;
     const float phi = normal_cdf(z, e);
     return fmaf(z * 0.3989422804014327f, e, phi);
   }
-  if constexpr (ACT == SMOE_ACT_GELU_TANH) {
-    // s + z s (1 - s) (2u)'; beyond |z| = 30 s is 0 or 1 to fp32, and the clamp keeps
-    // z^2 finite there
-    const float q = fminf(fmaxf(z, -30.0f), 30.0f);
-    const float s = sigmoid_f(gelu_tanh_2u(q));
-    const float slope = fmaf(q * s * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f * q, q, 1.0f), s);
-    return z == z ? slope : z;
+  if constexpr (ACT == SMOE_ACT_GELU_TANH) {  // s + z s (1 - s) (2u)'
+    z = clamp_nan(z, 30.0f);
+    const float s = sigmoid_f(gelu_tanh_2u(z));
+    return fmaf(z * s * (1.0f - s), 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f), s);
   }
   if constexpr (ACT == SMOE_ACT_SILU) {
+    z = clamp_nan(z, 128.0f);
     const float s = sigmoid_f(z);
     return s * fmaf(z, 1.0f - s, 1.0f);
   }
