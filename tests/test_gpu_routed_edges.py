@@ -1,5 +1,5 @@
 """Edges of sort_tokens, unsort_tokens and grouped_linear: pre-activations past the 16-bit
-range."""
+range, the activations over their whole range."""
 import math
 
 import pytest
@@ -14,6 +14,12 @@ ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
 def S():
     import swiftmoe_b200
     return swiftmoe_b200
+
+
+@pytest.fixture(scope="module")
+def K():
+    from swiftmoe_b200 import kernels
+    return kernels
 
 
 def gen(seed):
@@ -69,7 +75,56 @@ def slope64(z, name):
     return torch.ones_like(z), torch.ones_like(z)
 
 
+def relative(z, name):
+    """Relative error of an activation evaluated in fp32.  An exponential's argument of size A
+    is off by a few roundings, 2^-22 A; the rest of the evaluation by 2^-19."""
+    size = {"gelu": 0.5 * z * z, "gelu_tanh": two_u(z).abs(), "silu": z.abs()}.get(name)
+    if size is None:
+        return torch.zeros_like(z)
+    return 2.0 ** -19 + 2.0 ** -21 * size.clamp(max=200)
+
+
 # -------------------------------------------------------------------------- activations
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu"])
+def test_activation_over_its_whole_range(S, act, dtype, rows):
+    """z = the fp32 bias of a layer of zeros: relative accuracy down to the smallest normal
+    number, in the tails too."""
+    z = torch.cat([torch.linspace(-14, 14, 40000), torch.linspace(-100, 100, 8000),
+                   torch.tensor([0.0, -0.0, 1e-30, -1e-30, 3e4, -3e4, -1e20, -3e38])]).cuda()
+    n = z.numel()
+    out = S.grouped_linear(torch.zeros((rows, 8), dtype=dtype, device="cuda"),
+                           torch.zeros((1, n, 8), dtype=dtype, device="cuda"),
+                           torch.tensor([0, rows], dtype=torch.int32, device="cuda"), bias=z.view(1, n), activation=act)
+    z = z.double()
+    ref = act64(z, act)
+    big = ref.abs() > torch.finfo(dtype).max
+    assert torch.equal(out[:, big], ref[big].to(dtype).expand(rows, -1))
+    ref, z = ref[~big], z[~big]
+    err = relative(z, act) * ref.abs() + 2.0 ** -126
+    close(out[:, ~big], ref, half_step(ref, dtype) + (1 + torch.finfo(dtype).eps) * err)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["relu", "gelu"])
+def test_slope_of_every_16_bit_number(K, act, dtype):
+    z = torch.arange(-32768, 32768, device="cuda").to(torch.int16).view(dtype).view(64, 1024)
+    dz, _ = K.linear_act_bwd(torch.ones_like(z), torch.tensor([0, 64], dtype=torch.int32, device="cuda"), act, z)
+    assert torch.equal(dz.isnan() & ~z.isnan(), torch.zeros_like(z, dtype=torch.bool))
+    if act != "relu":
+        assert dz[z.isnan()].isnan().all()
+    assert (dz[z == math.inf] == 1).all() and (dz[z == -math.inf] == 0).all()
+    ok = z.isfinite()
+    z, dz = z[ok].double(), dz[ok]
+    ref, mag = slope64(z, act)
+    # beyond |z| = 200 every slope is 0 or 1 (and z d may overflow nowhere: d is 0)
+    far = z.abs() > 200
+    ref = torch.where(far, (z > 0).double(), ref)
+    mag = torch.where(far, ref, mag)
+    close(dz, ref, half_step(ref, dtype) + (1 + torch.finfo(dtype).eps) * (relative(z, act) * mag + 2.0 ** -126))
+
+
 @pytest.mark.parametrize("rows", [2, 40, 300])
 @pytest.mark.parametrize("act", ACTS)
 def test_finite_gradients_where_pre_activations_leave_fp16(S, act, rows):
