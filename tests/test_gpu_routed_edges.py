@@ -87,7 +87,7 @@ def relative(z, name):
 # -------------------------------------------------------------------------- activations
 @pytest.mark.parametrize("rows", [1, 3])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("act", ["none", "relu", "gelu"])
+@pytest.mark.parametrize("act", ACTS)
 def test_activation_over_its_whole_range(S, act, dtype, rows):
     """z = the fp32 bias of a layer of zeros: relative accuracy down to the smallest normal
     number, in the tails too."""
@@ -107,7 +107,7 @@ def test_activation_over_its_whole_range(S, act, dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("act", ["relu", "gelu"])
+@pytest.mark.parametrize("act", ACTS[1:])
 def test_slope_of_every_16_bit_number(K, act, dtype):
     z = torch.arange(-32768, 32768, device="cuda").to(torch.int16).view(dtype).view(64, 1024)
     dz, _ = K.linear_act_bwd(torch.ones_like(z), torch.tensor([0, 64], dtype=torch.int32, device="cuda"), act, z)
