@@ -174,7 +174,8 @@ SMOE_API int smoe_combine(const void* y, int dtype, const int32_t* slot_row, con
 SMOE_API int smoe_sort_rows(const void* x, int dtype, const int32_t* slot_row, const float* w, int T, int k, int d,
                             const int32_t* row_token, const int32_t* expert_offsets, int E, int64_t rows_cap,
                             void* rows, const void* y, float* dw, smoe_stream_t stream);
-/* smoe_dispatch_plan and smoe_sort_rows (no dw) in one call. */
+/* smoe_dispatch_plan and smoe_sort_rows (no dw) in one call.  The workspace may be the memory of
+ * `rows`: the plan is done with it before the rows are written. */
 SMOE_API int smoe_sort_tokens(const void* x, int dtype, const int32_t* idx, const float* w, int T, int k, int d, int E,
                               int capacity, int row_align, int32_t* expert_counts, int32_t* expert_offsets,
                               int32_t* slot_row, int32_t* row_token, int64_t rows_cap, void* rows, void* workspace,

@@ -209,11 +209,14 @@ def sort_tokens(x: torch.Tensor, idx: torch.Tensor, num_experts: int, w: Optiona
     need = lib.smoe_plan_workspace_size(T, k, E)
     if E < 1:
         raise L.SwiftMoEError("num_experts must be positive")
-    # the plan's arrays and its scratch from one allocation
-    counts, offsets, slot_row, row_token, ws = torch.empty(
-        2 * E + 1 + T * k + max(rows_cap, 1) + (need + 3) // 4, dtype=i32, device=dev).split_with_sizes(
-        (E, E + 1, T * k, max(rows_cap, 1), (need + 3) // 4))
+    # each array by itself: cut from one allocation (2 us less in a call) they would share a
+    # version counter, and keeping the counts would keep everything
+    counts, offsets = torch.empty(E, dtype=i32, device=dev), torch.empty(E + 1, dtype=i32, device=dev)
+    slot_row = torch.empty(T * k, dtype=i32, device=dev)
+    row_token = torch.empty(max(rows_cap, 1), dtype=i32, device=dev)
     rows = torch.empty((rows_cap, d), dtype=x.dtype, device=dev)
+    # the plan's scratch is used up before the last launch writes the rows
+    ws = rows if rows_cap * d * x.element_size() >= need else _workspace(dev, need)
     with _on(dev):
         L.check(lib.smoe_sort_tokens(x.data_ptr(), dt, idx.data_ptr(), L.ptr(w), T, k, d, E, capacity, row_align,
                                      counts.data_ptr(), offsets.data_ptr(), slot_row.data_ptr(), row_token.data_ptr(),

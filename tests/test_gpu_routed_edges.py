@@ -1,5 +1,6 @@
 """Edges of sort_tokens, unsort_tokens and grouped_linear: pre-activations past the 16-bit
-range, the activations over their whole range."""
+range, the activations over their whole range, plans that change between forward and
+backward."""
 import math
 
 import pytest
@@ -163,3 +164,35 @@ def test_finite_gradients_where_pre_activations_leave_fp16(S, act, rows):
                         (got[2][0], dz.sum(0), e.sum(0) + rows * 2.0 ** -23 * dz.abs().sum(0)), (got[3], do, 0 * do)):
         assert x.isfinite().all()
         close(x, ref, half_step(ref, x.dtype) * 1.01 + err)
+
+
+# ----------------------------------------------------------------------------- the plan
+def routed(S, capacity=0, align=1):
+    g = gen(5)
+    T, E, k, d = 60, 5, 2, 32
+    idx = torch.stack([torch.randperm(E, generator=g, device="cuda")[:k] for _ in range(T)]).to(torch.int32)
+    x = torch.randn((T, d), generator=g, device="cuda").bfloat16().requires_grad_()
+    w = torch.rand((T, k), generator=g, device="cuda").requires_grad_()
+    wt = (torch.randn((E, d, d), generator=g, device="cuda") / 6).bfloat16().requires_grad_()
+    rows, plan = S.sort_tokens(x, idx, E, weights=w, capacity=capacity, row_align=align)
+    return x, w, wt, rows, plan
+
+
+def test_load_counts_may_be_updated_before_the_backward(S):
+    def grads(change):
+        x, w, wt, rows, plan = routed(S)
+        out = S.unsort_tokens(S.grouped_linear(rows, wt, plan["offsets"]), plan, weights=w)
+        if change:
+            plan["counts"].add_(7).mul_(3)
+        return torch.autograd.grad(out, [x, w, wt], torch.ones_like(out))
+
+    assert all(torch.equal(p, q) for p, q in zip(grads(False), grads(True)))
+
+
+def test_plan_arrays_own_their_memory(S):
+    """Keeping one of them keeps no other one, nor the plan's scratch."""
+    plan = routed(S)[4]
+    arrays = [plan[n] for n in ("counts", "offsets", "slot_row", "row_token")]
+    assert len({t.untyped_storage().data_ptr() for t in arrays}) == 4
+    for t in arrays:
+        assert t.untyped_storage().nbytes() == t.numel() * 4
