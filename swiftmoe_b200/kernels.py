@@ -146,18 +146,17 @@ def combine(y: torch.Tensor, slot_row: torch.Tensor, w: torch.Tensor, T: int, k:
 
 
 def _plan_args(plan: dict, rows: int, w: Optional[torch.Tensor]):
-    """(slot_row, offsets, T, k) of a dispatch plan after checking that it fits `rows` rows
-    and w."""
-    slot_row, offsets, T, k = plan["slot_row"], plan["offsets"], plan["T"], plan["k"]
-    if slot_row.dtype != torch.int32 or offsets.dtype != torch.int32 or slot_row.numel() != T * k:
-        raise L.SwiftMoEError("not a dispatch plan: slot_row must be int32 [T*k], offsets int32")
+    """(slot_row, T, k) of a dispatch plan after checking that it fits `rows` rows and w."""
+    slot_row, T, k = plan["slot_row"], plan["T"], plan["k"]
+    if slot_row.dtype != torch.int32 or slot_row.numel() != T * k:
+        raise L.SwiftMoEError("not a dispatch plan: slot_row must be int32 [T*k]")
     if T * k > _MAX_INT:
         raise L.SwiftMoEError("a plan has at most 2^31 - 1 slots")
     if rows < plan["rows_cap"]:
         raise L.SwiftMoEError(f"the plan has up to {plan['rows_cap']} rows, the tensor only {rows}")
     if w is not None and (w.dtype != torch.float32 or w.shape != (T, k)):
         raise L.SwiftMoEError(f"weights must be float32 [{T}, {k}], got {w.dtype} {tuple(w.shape)}")
-    return slot_row, offsets, T, k
+    return slot_row, T, k
 
 
 def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, rows_cap: Optional[int] = None,
@@ -169,11 +168,13 @@ def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, 
     y[slot_row[t,j]]>: for x = the gradient of ``unsort_rows``' output and y = its rows
     these are its gradients."""
     rows_cap = plan["rows_cap"] if rows_cap is None else rows_cap
-    slot_row, offsets, T, k = _plan_args(plan, rows_cap, w)
-    row_token = plan["row_token"] if plan.get("row_align") != 1 else None
+    slot_row, T, k = _plan_args(plan, rows_cap, w)
+    offsets, row_token = plan["offsets"], plan["row_token"] if plan.get("row_align") != 1 else None
     dev = _device_of(x, slot_row, offsets, row_token, w, y)
     if x.dim() != 2 or x.shape[0] != T:
         raise L.SwiftMoEError(f"the plan is for {T} tokens, got x of shape {tuple(x.shape)}")
+    if offsets.dtype != torch.int32:
+        raise L.SwiftMoEError("not a dispatch plan: offsets must be int32")
     if row_token is not None and (row_token.dtype != torch.int32 or row_token.numel() < plan["rows_cap"]):
         raise L.SwiftMoEError("not a dispatch plan: row_token must be int32 [rows_cap]")
     d = x.shape[1]
@@ -238,7 +239,7 @@ def unsort_rows(y: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, r
         raise L.SwiftMoEError(f"rows must be [rows, d], got {tuple(y.shape)}")
     rows_cap, d = y.shape
     _columns(d)
-    slot_row, _, T, k = _plan_args(plan, rows_cap, w)
+    slot_row, T, k = _plan_args(plan, rows_cap, w)
     dev = _device_of(y, slot_row, w, residual, x)
     for name, t in (("residual", residual), ("x", x)):
         if t is not None and (t.dtype != y.dtype or t.shape != (T, d)):

@@ -31,44 +31,50 @@ def _grads_wanted(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def _sizes(plan: dict) -> dict:
+    """What a backward needs of a plan besides tensors, as it is now: the dict is the caller's."""
+    return {n: plan.get(n) for n in ("T", "k", "rows_cap", "row_align")}
+
+
 class _SortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, args, made):
         rows, plan = K.sort_tokens(x, args[0], args[1], w, args[2], args[3])
         made.append(plan)
-        ctx.plan = plan
-        ctx.save_for_backward(x if w is not None else None, w)
+        ctx.sizes = _sizes(plan)
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, w, plan["slot_row"])
         return rows
 
     @staticmethod
     @once_differentiable
     def backward(ctx, drows):
-        x, w = ctx.saved_tensors
-        drows = drows.contiguous()
+        x, w, slot_row = ctx.saved_tensors
+        drows, plan = drows.contiguous(), dict(ctx.sizes, slot_row=slot_row)
         if ctx.needs_input_grad[1]:
-            dx, dw = K.unsort_rows(drows, ctx.plan, w, x=x)
+            dx, dw = K.unsort_rows(drows, plan, w, x=x)
             return dx, dw, None, None
-        return K.unsort_rows(drows, ctx.plan, w), None, None, None
+        return K.unsort_rows(drows, plan, w), None, None, None
 
 
 class _UnsortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, w, residual, plan):
-        ctx.plan, ctx.rows_cap = plan, rows.shape[0]
-        ctx.save_for_backward(rows if w is not None else None, w, plan["slot_row"])
+        ctx.sizes, ctx.rows_cap = _sizes(plan), rows.shape[0]
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, w, plan["slot_row"], plan["offsets"],
+                              plan["row_token"] if plan.get("row_align") != 1 else None)
         return K.unsort_rows(rows, plan, w, residual)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        rows, w, _ = ctx.saved_tensors
+        rows, w, slot_row, offsets, row_token = ctx.saved_tensors
         need_rows, need_w, need_res, _ = ctx.needs_input_grad
-        dout = dout.contiguous()
+        dout, plan = dout.contiguous(), dict(ctx.sizes, slot_row=slot_row, offsets=offsets, row_token=row_token)
         drows = dw = None
         if need_w:
-            drows, dw = K.sort_rows(dout, ctx.plan, w, rows_cap=ctx.rows_cap, y=rows)
+            drows, dw = K.sort_rows(dout, plan, w, rows_cap=ctx.rows_cap, y=rows)
         elif need_rows:
-            drows = K.sort_rows(dout, ctx.plan, w, rows_cap=ctx.rows_cap)
+            drows = K.sort_rows(dout, plan, w, rows_cap=ctx.rows_cap)
         return drows if need_rows else None, dw, dout if need_res else None, None
 
 

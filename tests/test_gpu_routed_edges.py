@@ -196,3 +196,47 @@ def test_plan_arrays_own_their_memory(S):
     assert len({t.untyped_storage().data_ptr() for t in arrays}) == 4
     for t in arrays:
         assert t.untyped_storage().nbytes() == t.numel() * 4
+
+
+@pytest.mark.parametrize("name", ["slot_row", "offsets", "row_token"])
+@pytest.mark.parametrize("align", [1, 8])
+def test_a_plan_changed_in_place_is_not_used_for_gradients(S, name, align):
+    """What a backward reads of the plan is as it was in the forward, or the backward is refused."""
+    def run(change):
+        x, w, _, rows, plan = routed(S, align=align)
+        out = S.unsort_tokens(rows, plan, weights=w)
+        keep = plan[name].clone()
+        if change:
+            plan[name].zero_()
+        try:
+            return torch.autograd.grad(out, [x, w], torch.ones_like(out)), None
+        except RuntimeError as e:
+            plan[name].copy_(keep)
+            return None, str(e)
+
+    want, _ = run(False)
+    got, error = run(True)
+    if error is None:
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    else:
+        assert "modified by an inplace operation" in error
+    if name == "slot_row":
+        assert error is not None
+        # sort's own backward, too
+        x, w, _, rows, plan = routed(S, align=align)
+        plan["slot_row"].zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(rows, [x], torch.ones_like(rows))
+
+
+def test_a_plan_entry_replaced_before_the_backward_has_no_influence(S):
+    def grads(change):
+        x, w, _, rows, plan = routed(S)
+        out = S.unsort_tokens(rows, plan, weights=w)
+        if change:
+            plan["slot_row"] = torch.zeros_like(plan["slot_row"])
+            plan["offsets"] = torch.zeros_like(plan["offsets"])
+            plan["rows_cap"] = 1
+        return torch.autograd.grad(out, [x, w], torch.ones_like(out))
+
+    assert all(torch.equal(p, q) for p, q in zip(grads(False), grads(True)))
