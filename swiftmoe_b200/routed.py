@@ -14,6 +14,9 @@ accumulates into leaves whose stream torch recorded outside the capture, which t
 not allow; drop the eager graph's outputs before capturing, or call the ``kernels``
 functions that the backward consists of.)
 
+Reverse mode only: a tensor with a forward-mode tangent is refused, and so is a second
+derivative.
+
 The reference's pieces are forward-only: models/ultimate_moe.py:118-125 (dispatch), 145-155
 (combine), 237-250 and models/baseline_moe.py:151-162 (experts).
 """
@@ -22,12 +25,18 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
+from . import _lib as L
 from . import kernels as K
 
 
 def _grads_wanted(*ts) -> bool:
+    # Tangents are refused here: the kernels read memory, where a dual tensor's is not, and
+    # such tensors need not have requires_grad set.  (_current_level: -1 outside a dual level)
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise L.SwiftMoEError("forward-mode derivatives of the routed rows are not supported")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
