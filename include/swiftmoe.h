@@ -163,7 +163,8 @@ SMOE_API int smoe_combine(const void* y, int dtype, const int32_t* slot_row, con
  * rows_cap rows becomes zero: those from expert_offsets[E] on and, when row_token is
  * given (plans with row_align > 1), the alignment padding.  With dw != NULL (needs w) also
  * dw[t,j] = <x[t,:], y[slot_row[t,j],:]> (0 for slots without a row): called with x = the
- * gradient of smoe_unsort_rows' output and y = its rows, this is that call's gradient.
+ * gradient of smoe_unsort_rows' output and y = its rows, this is that call's gradient.  With
+ * rows == NULL (expert_offsets and row_token unused) it is dw alone, in either direction.
  *
  * smoe_unsort_rows: out[t,:] = sum_j w[t,j] * y[slot_row[t,j],:] (+ residual[t,:]).  With
  * dw != NULL (needs w) also dw[t,j] = <x[t,:], y[slot_row[t,j],:]>: the gradient of smoe_sort_rows,

@@ -761,7 +761,7 @@ cudaError_t launch_sort_rows(const void* x, const int32_t* sr, const float* w, i
                              const int32_t* row_token, const int32_t* offsets, int E, int64_t rows_cap, void* out,
                              const void* y, float* dw, cudaStream_t st) {
   // enough blocks for the tokens and, should most rows be of no slot, for clearing them
-  const unsigned fill = (unsigned)std::min<int64_t>(cdiv(rows_cap * (d / VEC), 8 * rows::THREADS), device_sms());
+  const unsigned fill = out ? (unsigned)std::min<int64_t>(cdiv(rows_cap * (d / VEC), 8 * rows::THREADS), device_sms()) : 1u;
   const unsigned grid = std::max(token_grid(T_, WPT, 64), fill);
 #define SMOE_SORT(HW, DOT)                                                                                          \
   return launch_k(rows::sort_rows_kernel<T, VEC, WPT, HW, DOT>, grid, rows::THREADS, 0, st, (const T*)x, sr, w, T_, k, \
@@ -1172,7 +1172,9 @@ int smoe_sort_rows(const void* x, int dtype, const int32_t* slot_row, const floa
   if (es == 0 || T < 0 || k < 1 || d < 1 || E < 1 || rows_cap < 0) return SMOE_ERR_INVALID;
   if (k > rows::MAX_K || d > kMaxCols || rows_cap > kMaxRows) return SMOE_ERR_UNSUPPORTED;
   if (T == 0 && rows_cap == 0) return SMOE_OK;
-  if (!expert_offsets || (rows_cap > 0 && !rows) || (T > 0 && (!x || !slot_row)) || (dw && (!w || (rows_cap > 0 && !y))))
+  if (!rows && dw && T == 0) return SMOE_OK;
+  if ((rows_cap > 0 && !rows && !dw) || (!expert_offsets && (rows || !dw)) || (T > 0 && (!x || !slot_row)) ||
+      (dw && (!w || (rows_cap > 0 && !y))))
     return SMOE_ERR_INVALID;
   const int vec = row_vec(es, d, {x, rows, dw ? y : nullptr}), wpt = token_warps(T, d / vec);
   cudaStream_t st = (cudaStream_t)stream;

@@ -110,7 +110,9 @@ __device__ __forceinline__ void store_dots(float my, bool live, int64_t t, int k
 }
 
 // sort (and the gradient of unsort).  WPT warps share a token's columns.  DOT > 0: also
-// dw[t, j] = <x_t, y[r(t,j)]>, 0 for slots without a row.
+// dw[t, j] = <x_t, y[r(t,j)]>, 0 for slots without a row; rows may then be null: dw alone, the
+// same operation in both directions (32768 x 8 fp16 rows of 2048: 182 us, 222 and 348 together
+// with unsort's and sort's other output; a form of unsort without its output took 210).
 template <typename T, int VEC, int WPT, bool HAS_W, int DOT>
 __global__ void __launch_bounds__(THREADS) sort_rows_kernel(const T* __restrict__ x, const int32_t* __restrict__ slot_row,
                                                             const float* __restrict__ w, int T_, int k, int d,
@@ -153,14 +155,16 @@ __global__ void __launch_bounds__(THREADS) sort_rows_kernel(const T* __restrict_
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (!FULL && c0 + u * STEP >= nv) continue;
-          T* dst = rows + r * d + (int64_t)(c0 + u * STEP) * VEC;
-          if constexpr (HAS_W) {
-            Piece<T, VEC> o;
+          if (DOT == 0 || rows != nullptr) {
+            T* dst = rows + r * d + (int64_t)(c0 + u * STEP) * VEC;
+            if constexpr (HAS_W) {
+              Piece<T, VEC> o;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o.e[i] = Num<T>::from_f(wj * v[u].f(i));
-            o.store(dst);
-          } else {
-            v[u].store(dst);
+              for (int i = 0; i < VEC; ++i) o.e[i] = Num<T>::from_f(wj * v[u].f(i));
+              o.store(dst);
+            } else {
+              v[u].store(dst);
+            }
           }
           if constexpr (DOT > 0)
 #pragma unroll
@@ -185,6 +189,7 @@ __global__ void __launch_bounds__(THREADS) sort_rows_kernel(const T* __restrict_
     }
     if constexpr (DOT > 0) store_dots<WPT>(dots.total(), live, t, k, dw);
   }
+  if (DOT > 0 && rows == nullptr) return;
   // rows of no slot become zeros: the rows from the plan's total on, all threads together,
   const int64_t total = min((int64_t)max(offsets[E], 0), rows_cap);
   Piece<T, VEC> z;

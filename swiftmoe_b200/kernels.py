@@ -160,20 +160,22 @@ def _plan_args(plan: dict, rows: int, w: Optional[torch.Tensor]):
 
 
 def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, rows_cap: Optional[int] = None,
-              y: Optional[torch.Tensor] = None):
+              y: Optional[torch.Tensor] = None, only_dw: bool = False):
     """rows [rows_cap, d] with rows[slot_row[t,j]] = (w[t,j] *) x[t]; all other rows (padding,
     rows behind the last expert's) are zero.  rows_cap: the plan's unless given.
 
     With ``y`` [rows_cap, d] (needs w) returns (rows, dw [T,k] fp32), dw[t,j] = <x[t],
     y[slot_row[t,j]]>: for x = the gradient of ``unsort_rows``' output and y = its rows
-    these are its gradients."""
+    these are its gradients.  ``only_dw``: dw alone, no rows are written (for x = the input of
+    ``sort_rows`` and y = its rows' gradient it is that direction's)."""
     rows_cap = plan["rows_cap"] if rows_cap is None else rows_cap
     slot_row, T, k = _plan_args(plan, rows_cap, w)
-    offsets, row_token = plan["offsets"], plan["row_token"] if plan.get("row_align") != 1 else None
+    offsets = None if only_dw else plan["offsets"]
+    row_token = None if only_dw or plan.get("row_align") == 1 else plan["row_token"]
     dev = _device_of(x, slot_row, offsets, row_token, w, y)
     if x.dim() != 2 or x.shape[0] != T:
         raise L.SwiftMoEError(f"the plan is for {T} tokens, got x of shape {tuple(x.shape)}")
-    if offsets.dtype != torch.int32:
+    if offsets is not None and offsets.dtype != torch.int32:
         raise L.SwiftMoEError("not a dispatch plan: offsets must be int32")
     if row_token is not None and (row_token.dtype != torch.int32 or row_token.numel() < plan["rows_cap"]):
         raise L.SwiftMoEError("not a dispatch plan: row_token must be int32 [rows_cap]")
@@ -181,14 +183,16 @@ def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, 
     _columns(d)
     if y is not None and (w is None or y.dtype != x.dtype or y.shape != (rows_cap, d)):
         raise L.SwiftMoEError("y needs weights, x's dtype and shape [rows_cap, d]")
+    if only_dw and y is None:
+        raise L.SwiftMoEError("the weights' gradient needs y")
     dt = L.dtype_code(x.dtype)
-    rows = torch.empty((rows_cap, d), dtype=x.dtype, device=dev)
+    rows = None if only_dw else torch.empty((rows_cap, d), dtype=x.dtype, device=dev)
     dw = torch.empty((T, k), dtype=torch.float32, device=dev) if y is not None else None
     with _on(dev):
         L.check(L.load().smoe_sort_rows(x.data_ptr(), dt, slot_row.data_ptr(), L.ptr(w), T, k, d, L.ptr(row_token),
-                                        offsets.data_ptr(), offsets.numel() - 1, rows_cap, rows.data_ptr(), L.ptr(y),
-                                        L.ptr(dw), L.stream_handle(dev)), "smoe_sort_rows")
-    return rows if y is None else (rows, dw)
+                                        L.ptr(offsets), 1 if only_dw else offsets.numel() - 1, rows_cap, L.ptr(rows),
+                                        L.ptr(y), L.ptr(dw), L.stream_handle(dev)), "smoe_sort_rows")
+    return dw if only_dw else rows if y is None else (rows, dw)
 
 
 def sort_tokens(x: torch.Tensor, idx: torch.Tensor, num_experts: int, w: Optional[torch.Tensor] = None,

@@ -59,9 +59,11 @@ class _SortTokens(torch.autograd.Function):
     def backward(ctx, drows):
         x, w, slot_row = ctx.saved_tensors
         drows, plan = drows.contiguous(), dict(ctx.sizes, slot_row=slot_row)
-        if ctx.needs_input_grad[1]:
-            dx, dw = K.unsort_rows(drows, plan, w, x=x)
-            return dx, dw, None, None
+        need_x, need_w = ctx.needs_input_grad[:2]
+        if need_w and not need_x:
+            return None, K.sort_rows(x, plan, w, rows_cap=drows.shape[0], y=drows, only_dw=True), None, None
+        if need_w:
+            return *K.unsort_rows(drows, plan, w, x=x), None, None
         return K.unsort_rows(drows, plan, w), None, None, None
 
 
@@ -80,11 +82,13 @@ class _UnsortTokens(torch.autograd.Function):
         need_rows, need_w, need_res, _ = ctx.needs_input_grad
         dout, plan = dout.contiguous(), dict(ctx.sizes, slot_row=slot_row, offsets=offsets, row_token=row_token)
         drows = dw = None
-        if need_w:
+        if need_w and not need_rows:
+            dw = K.sort_rows(dout, plan, w, rows_cap=ctx.rows_cap, y=rows, only_dw=True)
+        elif need_w:
             drows, dw = K.sort_rows(dout, plan, w, rows_cap=ctx.rows_cap, y=rows)
         elif need_rows:
             drows = K.sort_rows(dout, plan, w, rows_cap=ctx.rows_cap)
-        return drows if need_rows else None, dw, dout if need_res else None, None
+        return drows, dw, dout if need_res else None, None
 
 
 class _GroupedLinear(torch.autograd.Function):

@@ -1,6 +1,7 @@
 """Edges of sort_tokens, unsort_tokens and grouped_linear: pre-activations past the 16-bit
 range, the activations over their whole range, plans that change between forward and
-backward."""
+backward, gradients of some inputs only."""
+import gc
 import math
 
 import pytest
@@ -240,3 +241,40 @@ def test_a_plan_entry_replaced_before_the_backward_has_no_influence(S):
         return torch.autograd.grad(out, [x, w], torch.ones_like(out))
 
     assert all(torch.equal(p, q) for p, q in zip(grads(False), grads(True)))
+
+
+# ------------------------------------------------------------------ gradients of some inputs
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,d,E,k,cap,align", [(60, 32, 5, 2, 0, 1), (2500, 264, 16, 4, 500, 8), (33, 1027, 40, 32, 3, 4),
+                                               (700, 1032, 12, 10, 0, 1)])
+def test_gradient_of_the_weights_alone(S, dtype, T, d, E, k, cap, align):
+    g = gen(T)
+    idx = torch.stack([torch.randperm(E, generator=g, device="cuda")[:k] for _ in range(T)]).to(torch.int32)
+    w = torch.rand((T, k), generator=g, device="cuda").requires_grad_()
+    x = torch.randn((T, d), generator=g, device="cuda").to(dtype)
+
+    def both(call, other, dout, terms=None):
+        o = other.detach().requires_grad_()
+        want = torch.autograd.grad(call(o), [o, w], dout)[1]
+        out = call(other.detach())
+        gc.collect()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        (got,) = torch.autograd.grad(out, [w], dout)
+        peak = torch.cuda.max_memory_allocated() - before
+        if terms is None:
+            assert torch.equal(got, want)
+        else:   # the same products in another fp32 order: a lane's own terms, then lanes and warps
+            x_, y_, sr = terms
+            mag = torch.where((sr >= 0).unsqueeze(2), y_.double()[sr.clamp(min=0)], 0.0).mul(x_.double().unsqueeze(1))
+            close(got, want.double(), 2 * (d / 32 + 16) * 2.0 ** -24 * mag.abs().sum(2))
+        return peak
+
+    rows, plan = S.sort_tokens(x, idx, E, capacity=cap, row_align=align)
+    drows, dout = torch.randn_like(rows), torch.randn_like(x)
+    dw_bytes = -(-T * k * 4 // 512) * 512
+    # the gradient itself is all that is allocated
+    assert both(lambda t: S.sort_tokens(t, idx, E, weights=w, capacity=cap, row_align=align)[0], x, drows,
+                (x, drows, plan["slot_row"].view(T, k).long())) <= dw_bytes
+    assert both(lambda t: S.unsort_tokens(t, plan, weights=w), rows, dout) <= dw_bytes
