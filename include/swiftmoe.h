@@ -261,8 +261,8 @@ SMOE_API int smoe_linear_wgrad(const void* dz, const void* A, int dtype, const i
 /* The three in one call: the gradients of smoe_grouped_linear's output (without its residual,
  * whose gradient is dout) that are asked for -- dA [rows_cap, K], dW [G, N, K], dbias [G, N],
  * each NULL or not -- from dout [rows_cap, N] and what the forward had (W in SMOE_W_NK, preact
- * unless act is SMOE_ACT_NONE).  Rows of no group have no influence, and dA 0.  `grads` of the
- * size query: SMOE_GRAD_* of the outputs asked for.                                      */
+ * unless act is SMOE_ACT_NONE; A may be NULL without dW, W without dA).  Rows of no group have
+ * no influence, and dA 0.  `grads` of the size query: SMOE_GRAD_* of the outputs asked for. */
 #define SMOE_GRAD_A 1
 #define SMOE_GRAD_W 2
 #define SMOE_GRAD_BIAS 4

@@ -365,34 +365,37 @@ def linear_wgrad(dz: torch.Tensor, A: torch.Tensor, offsets: torch.Tensor,
     return dW
 
 
-def grouped_linear_bwd(dout: torch.Tensor, A: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, activation: str,
-                       preact: Optional[torch.Tensor] = None, *, need_a: bool = True, need_w: bool = True,
-                       bias_dtype: Optional[torch.dtype] = None):
+def grouped_linear_bwd(dout: torch.Tensor, A: Optional[torch.Tensor], W: Optional[torch.Tensor], offsets: torch.Tensor,
+                       activation: str, preact: Optional[torch.Tensor] = None, *, need_a: bool = True,
+                       need_w: bool = True, bias_dtype: Optional[torch.dtype] = None):
     """(dA, dW, dbias) of ``grouped_linear``'s output (W [G, N, K]), None for those not asked for:
     ``linear_act_bwd``, ``grouped_linear`` with the weights as they are and ``linear_wgrad`` in
-    one library call."""
+    one library call.  A is used for dW only and W for dA only; either may be None without it."""
+    if (need_w and A is None) or (need_a and W is None) or (A is None and W is None):
+        raise L.SwiftMoEError("dW needs A, dA needs W (for dbias alone: linear_act_bwd)")
     dev = _device_of(dout, A, W, offsets, preact)
-    act, dt = _act_code(activation), _linear_dtype(A)
-    if A.dim() != 2 or W.dim() != 3 or W.dtype != A.dtype or dout.dtype != A.dtype:
+    act, dt = _act_code(activation), _linear_dtype(dout)
+    if dout.dim() != 2 or (A is not None and (A.dim() != 2 or A.dtype != dout.dtype)) or (
+            W is not None and (W.dim() != 3 or W.dtype != dout.dtype)):
         raise L.SwiftMoEError("dout, A [rows, K] and W [G, N, K] must have the same dtype")
-    rows_cap, Kd = A.shape
-    G, N, K2 = W.shape
-    if K2 != Kd or dout.shape != (rows_cap, N):
+    rows_cap, N = dout.shape
+    G, Kd = offsets.numel() - 1, A.shape[1] if W is None else W.shape[2]
+    if (A is not None and A.shape != (rows_cap, Kd)) or (W is not None and W.shape[1] != N):
         raise L.SwiftMoEError("dout must be [rows, N], A [rows, K]")
     _columns(N, Kd)
-    _group_offsets(offsets, G)
-    if act and (preact is None or preact.dtype != A.dtype or preact.shape != dout.shape):
+    _group_offsets(offsets, G if W is None else W.shape[0])
+    if act and (preact is None or preact.dtype != dout.dtype or preact.shape != dout.shape):
         raise L.SwiftMoEError("preact must have dout's dtype and shape")
     lib = L.load()
-    dA = torch.empty((rows_cap, Kd), dtype=A.dtype, device=dev) if need_a else None
-    dW = torch.empty((G, N, Kd), dtype=A.dtype, device=dev) if need_w else None
+    dA = torch.empty((rows_cap, Kd), dtype=dout.dtype, device=dev) if need_a else None
+    dW = torch.empty((G, N, Kd), dtype=dout.dtype, device=dev) if need_w else None
     dbias = torch.empty((G, N), dtype=bias_dtype, device=dev) if bias_dtype is not None else None
     with _on(dev):
         need = lib.smoe_grouped_linear_bwd_workspace_size(
             act, need_a * L.SMOE_GRAD_A + need_w * L.SMOE_GRAD_W + (dbias is not None) * L.SMOE_GRAD_BIAS, dt, rows_cap, G,
             N, Kd)
         ws = _workspace(dev, need) if need else None
-        L.check(lib.smoe_grouped_linear_bwd(dout.data_ptr(), A.data_ptr(), W.data_ptr(), L.ptr(preact), act, dt,
+        L.check(lib.smoe_grouped_linear_bwd(dout.data_ptr(), L.ptr(A), L.ptr(W), L.ptr(preact), act, dt,
                                             offsets.data_ptr(), G, rows_cap, N, Kd, L.ptr(dA), L.ptr(dW), L.ptr(dbias),
                                             L.dtype_code(bias_dtype) if dbias is not None else dt, L.ptr(ws), need,
                                             L.stream_handle(dev)), "smoe_grouped_linear_bwd")

@@ -94,11 +94,12 @@ class _UnsortTokens(torch.autograd.Function):
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, weight, bias, residual, offsets, activation):
-        keep = activation != "none" and any(ctx.needs_input_grad[:3])
+        need_a, need_w, need_b, _ = ctx.needs_input_grad[:4]
+        keep = activation != "none" and (need_a or need_w or need_b)
         z = torch.empty((a.shape[0], weight.shape[1]), dtype=a.dtype, device=a.device) if keep else None
         out = K.grouped_linear(a, weight, offsets, bias, activation, residual, preact=z)
-        ctx.activation, ctx.bias_dtype = activation, bias.dtype if bias is not None else None
-        ctx.save_for_backward(a, weight, offsets, z)
+        ctx.activation, ctx.bias_dtype = activation, bias.dtype if need_b else None
+        ctx.save_for_backward(a if need_w else None, weight if need_a else None, offsets, z)
         return out
 
     @staticmethod
@@ -110,9 +111,11 @@ class _GroupedLinear(torch.autograd.Function):
         if dout.data_ptr() % 16:   # a piece of a larger gradient: the kernels load 16 bytes at a time
             dout = dout.clone()
         da = dw = db = None
-        if need_a or need_w or need_b:
+        if need_a or need_w:
             da, dw, db = K.grouped_linear_bwd(dout, a, weight, offsets, ctx.activation, z, need_a=need_a, need_w=need_w,
-                                              bias_dtype=ctx.bias_dtype if need_b else None)
+                                              bias_dtype=ctx.bias_dtype)
+        elif need_b:
+            _, db = K.linear_act_bwd(dout, offsets, ctx.activation, z, ctx.bias_dtype)
         return da, dw, db, dout if need_res else None, None, None
 
 

@@ -3,6 +3,7 @@ range, the activations over their whole range, plans that change between forward
 backward, gradients of some inputs only."""
 import gc
 import math
+import weakref
 
 import pytest
 import torch
@@ -278,3 +279,25 @@ def test_gradient_of_the_weights_alone(S, dtype, T, d, E, k, cap, align):
     assert both(lambda t: S.sort_tokens(t, idx, E, weights=w, capacity=cap, row_align=align)[0], x, drows,
                 (x, drows, plan["slot_row"].view(T, k).long())) <= dw_bytes
     assert both(lambda t: S.unsort_tokens(t, plan, weights=w), rows, dout) <= dw_bytes
+
+
+@pytest.mark.parametrize("needs", ["a", "w", "b", "r"])
+def test_grouped_linear_keeps_what_its_gradients_need(S, needs):
+    g = gen(1)
+    off = torch.tensor([0, 30, 50], dtype=torch.int32, device="cuda")
+
+    def made():
+        t = dict(a=torch.randn((50, 64), generator=g, device="cuda"), w=torch.randn((2, 24, 64), generator=g, device="cuda"),
+                 b=torch.randn((2, 24), generator=g, device="cuda"), r=torch.randn((50, 24), generator=g, device="cuda"))
+        return {n: v.bfloat16() for n, v in t.items()}
+
+    t = made()
+    t[needs].requires_grad_()
+    leaf, dead = t[needs], {n: weakref.ref(v) for n, v in t.items() if n != needs}
+    out = S.grouped_linear(t["a"], t["w"], off, bias=t["b"], activation="gelu", residual=t["r"])
+    del t
+    gc.collect()
+    kept = {n for n, v in dead.items() if v() is not None}
+    assert kept == {"a": {"w"}, "w": {"a"}, "b": set(), "r": set()}[needs]
+    (grad,) = torch.autograd.grad(out, [leaf], torch.ones_like(out))
+    assert grad.shape == leaf.shape
