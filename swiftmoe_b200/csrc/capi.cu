@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <initializer_list>
@@ -743,12 +744,22 @@ cudaError_t launch_act_bwd(const void* dout, const void* z, void* dz, int act, c
 }
 
 // ------------------------------------------------------------------ tokens <-> rows
-// One warp per token, or the eight warps of a block for few tokens with long rows.  Sort with
-// gradient of the weights / unsort, one warp against eight: 6.9 / 8.2 against 7.3 / 5.2 us
-// for 1000 x 2 bf16 rows of 4096, 9.3 / 10.0 against 12.5 / 8.5 for 2000, 10.4 / 14.0 against
-// 9.9 / 8.0 for 1537 x 3 fp32 rows of 1027 single elements, 6.6 / 3.5 against 12.9 / 8.8 for
-// 4000 x 2 rows of 64 pieces.
-int token_warps(int T, int64_t pieces) { return T < 12 * device_sms() && pieces >= 128 ? 8 : 1; }
+// One warp per token, or the eight warps of a block for few tokens with long rows: below
+// `per_sm` tokens per SM.  Where the two cross, from a sweep of 16 to 6000 tokens over rows of
+// 128 to 1024 16-byte pieces and 1 to 8 slots: sort near 16 tokens per SM whatever the rows (one
+// warp / eight, 4096 x 2 bf16: 5.0 / 4.7 us for 1000 tokens, 7.0 / 6.8 for 1776, 14.3 / 17.2
+// for 4000), with dw near 7 (7.1 / 5.6 for 600, 7.3 / 7.0 for 1000, 9.7 / 13.0 for 2000).
+// unsort's single warp waits for its k rows in turn, but eight warps a token reach less of the
+// memory's rate the more slots there are: it crosses at 3 to 7 tokens per SM for 32 pieces per
+// slot (1024 x 4 bf16: 3.6 / 2.8 for 300, 4.2 / 6.1 for 1400), at 18 for 256 (4096 x 2 bf16: 7.8 /
+// 7.3 for 2000, 14.9 / 16.8 for 4000) and above 30 for 1024 -- about the root of their number,
+// three quarters of it with dw.  Rows of less than half a block's pieces keep one warp: 6.6
+// (sort with dw) and 3.5 against 12.9 and 8.8 for 4000 x 2 rows of 64.
+int token_warps(int T, int64_t pieces, double per_sm) { return pieces >= 128 && T < per_sm * device_sms() ? 8 : 1; }
+double sort_per_sm(bool dw) { return dw ? 6 : 12; }
+double unsort_per_sm(int64_t row_bytes, int k, bool dw) {
+  return std::min(32.0, std::sqrt((double)row_bytes / (16 * k))) * (dw ? 0.75 : 1);
+}
 // waves: blocks per SM at most.  sort hands its tokens to 64 (222 us with 8, 193 with 64 for
 // 32768 x 8 fp16 rows of 2048: short blocks even out the end), unsort keeps 8 resident ones.
 unsigned token_grid(int T, int wpt, int waves) {
@@ -1176,7 +1187,7 @@ int smoe_sort_rows(const void* x, int dtype, const int32_t* slot_row, const floa
   if ((rows_cap > 0 && !rows && !dw) || (!expert_offsets && (rows || !dw)) || (T > 0 && (!x || !slot_row)) ||
       (dw && (!w || (rows_cap > 0 && !y))))
     return SMOE_ERR_INVALID;
-  const int vec = row_vec(es, d, {x, rows, dw ? y : nullptr}), wpt = token_warps(T, d / vec);
+  const int vec = row_vec(es, d, {x, rows, dw ? y : nullptr}), wpt = token_warps(T, d / vec, sort_per_sm(dw != nullptr));
   cudaStream_t st = (cudaStream_t)stream;
 #define SMOE_ROWS_LAUNCH(TY, VV, WW) \
   (launch_sort_rows<TY, VV, WW>(x, slot_row, w, T, k, d, row_token, expert_offsets, E, rows_cap, rows, y, dw, st))
@@ -1210,7 +1221,8 @@ int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const fl
   if (k > rows::MAX_K || d > kMaxCols || rows_cap > kMaxRows) return SMOE_ERR_UNSUPPORTED;
   if (T == 0) return SMOE_OK;
   if (!slot_row || !out || (rows_cap > 0 && !y) || (dw && (!w || !x))) return SMOE_ERR_INVALID;
-  const int vec = row_vec(es, d, {y, out, residual, dw ? x : nullptr}), wpt = token_warps(T, d / vec);
+  const int vec = row_vec(es, d, {y, out, residual, dw ? x : nullptr});
+  const int wpt = token_warps(T, d / vec, unsort_per_sm((int64_t)d * es, k, dw != nullptr));
   cudaStream_t st = (cudaStream_t)stream;
 #define SMOE_ROWS_LAUNCH(TY, VV, WW) \
   (launch_unsort_rows<TY, VV, WW>(y, slot_row, w, T, k, d, rows_cap, residual, out, x, dw, st))
