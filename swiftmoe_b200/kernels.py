@@ -44,6 +44,7 @@ def _device_of(first: torch.Tensor, *ts) -> torch.device:
 
 _HERE = nullcontext()
 _MAX_INT, _MAX_COLS = 2**31 - 1, 2**30   # what the library's int arguments hold; its columns
+_MAX_EXPERTS, _MAX_ALIGN = 4096, 1024    # a dispatch plan's limits
 
 
 def _columns(*n: int):
@@ -210,10 +211,12 @@ def sort_tokens(x: torch.Tensor, idx: torch.Tensor, num_experts: int, w: Optiona
     if T * k > _MAX_INT:
         raise L.SwiftMoEError("a plan has at most 2^31 - 1 slots")
     _columns(d)
+    # checked here: the library's int arguments would keep the low 32 bits alone
+    if not (1 <= E <= _MAX_EXPERTS and 1 <= row_align <= _MAX_ALIGN):
+        raise L.SwiftMoEError(f"num_experts must be 1 .. {_MAX_EXPERTS}, row_align 1 .. {_MAX_ALIGN}: got {E}, {row_align}")
+    capacity = max(0, min(capacity, _MAX_INT))
     rows_cap = lib.smoe_plan_rows_cap(T, k, E, capacity, row_align)
     need = lib.smoe_plan_workspace_size(T, k, E)
-    if E < 1:
-        raise L.SwiftMoEError("num_experts must be positive")
     # each array by itself: cut from one allocation (2 us less in a call) they would share a
     # version counter, and keeping the counts would keep everything
     counts, offsets = torch.empty(E, dtype=i32, device=dev), torch.empty(E + 1, dtype=i32, device=dev)

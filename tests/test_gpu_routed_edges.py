@@ -301,3 +301,17 @@ def test_grouped_linear_keeps_what_its_gradients_need(S, needs):
     assert kept == {"a": {"w"}, "w": {"a"}, "b": set(), "r": set()}[needs]
     (grad,) = torch.autograd.grad(out, [leaf], torch.ones_like(out))
     assert grad.shape == leaf.shape
+
+
+# ----------------------------------------------------------------------------- refusals
+def test_sizes_past_32_bits(S):
+    from swiftmoe_b200._lib import SwiftMoEError
+    x, idx = torch.randn((6, 16), device="cuda").bfloat16(), torch.zeros((6, 2), dtype=torch.int32, device="cuda")
+    big = 1 << 32
+    for kw in (dict(num_experts=big + 4), dict(num_experts=0), dict(num_experts=4097), dict(num_experts=4, row_align=big + 1),
+               dict(num_experts=4, row_align=0), dict(num_experts=4, row_align=1025)):
+        with pytest.raises(SwiftMoEError):
+            S.sort_tokens(x, idx, **kw)
+    # more than every slot: all of them are kept
+    rows, plan = S.sort_tokens(x, idx, 4, capacity=big + 5)
+    assert plan["rows_cap"] == 12 and torch.equal(rows, x.repeat_interleave(2, 0))
