@@ -230,10 +230,11 @@ SMOE_API int smoe_grouped_gemm_rows(const void* A, const void* B, const void* B3
  * Rows of no group -- before offsets[0] or from offsets[G] on -- are left as they were, or,
  * with fill != 0, become residual (zeros without one).  offsets are non-decreasing and live
  * in device memory; they are clamped into [0, rows_cap].  bf16 / fp16, N and K multiples of
- * 8 up to 2^30, 16-byte aligned pointers, G <= 1024, rows_cap < 2^31 - 65535; C must not
- * overlap A.  At most 2 rows stream the weights on the SIMT
- * pipes (SMOE_W_NK), everything else runs on tcgen05 tensor cores; launches of few tiles
- * split K over otherwise idle SMs through the workspace (its size may be 0).
+ * 8 up to 2^30, 16-byte aligned pointers, G <= 1024, rows_cap < 2^31 - 65535.  C may be
+ * the residual, but must not overlap A, W or another part of the residual; preact must not
+ * overlap any of them.  rows_cap <= 2 streams the weights on the SIMT pipes (SMOE_W_NK),
+ * everything else runs on tcgen05 tensor cores; launches of few tiles split K over otherwise
+ * idle SMs through the workspace (its size may be 0).
  * Replaces: nn.Linear experts with a bias around models/baseline_moe.py:151-162 (the
  * reference's own are bias-free and linear).                                           */
 SMOE_API size_t smoe_grouped_linear_workspace_size(int64_t rows_cap, int N, int K, int G, int w_layout);

@@ -96,6 +96,8 @@ class _GroupedLinear(torch.autograd.Function):
     def forward(ctx, a, weight, bias, residual, offsets, activation):
         need_a, need_w, need_b, _ = ctx.needs_input_grad[:4]
         keep = activation != "none" and (need_a or need_w or need_b)
+        if a.dim() != 2 or weight.dim() != 3:
+            raise L.SwiftMoEError("a must be [rows, K], weight [G, N, K]")
         z = torch.empty((a.shape[0], weight.shape[1]), dtype=a.dtype, device=a.device) if keep else None
         out = K.grouped_linear(a, weight, offsets, bias, activation, residual, preact=z)
         ctx.activation, ctx.bias_dtype = activation, bias.dtype if need_b else None

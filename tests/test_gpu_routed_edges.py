@@ -315,3 +315,36 @@ def test_sizes_past_32_bits(S):
     # more than every slot: all of them are kept
     rows, plan = S.sort_tokens(x, idx, 4, capacity=big + 5)
     assert plan["rows_cap"] == 12 and torch.equal(rows, x.repeat_interleave(2, 0))
+
+
+def test_shapes_and_overlaps_are_refused_as_such(S, K):
+    from swiftmoe_b200._lib import SwiftMoEError
+    n = lambda *s: torch.randn(s, device="cuda").bfloat16()  # noqa: E731
+    a, w, r, off = n(12, 16), n(2, 16, 16), n(12, 16), torch.tensor([0, 5, 12], dtype=torch.int32, device="cuda")
+    both = n(18, 16)
+    wg = w.clone().requires_grad_()
+
+    def refused(f):
+        with pytest.raises(SwiftMoEError):
+            f()
+
+    refused(lambda: S.grouped_linear(a[0], wg, off))                          # the same with and without gradients
+    refused(lambda: S.grouped_linear(a[0], w, off))
+    refused(lambda: S.grouped_linear(a, wg[0], off))
+    refused(lambda: S.grouped_linear(a, wg[0, 0], off))
+    refused(lambda: K.linear_act_bwd(a[0], off, "none"))
+    refused(lambda: K.linear_act_bwd(a, off[:0], "none", bias_dtype=torch.bfloat16))
+    refused(lambda: K.linear_wgrad(a, r, off[:0]))
+    refused(lambda: K.linear_wgrad(a, r, off[:1]))
+    refused(lambda: K.grouped_linear_bwd(r, None, None, off, "none", need_a=False, need_w=False))
+    refused(lambda: K.grouped_linear_bwd(r, None, w, off, "none"))
+    refused(lambda: K.grouped_linear_bwd(r, a, None, off, "none"))
+    refused(lambda: K.grouped_linear(a, w, off, out=a))
+    refused(lambda: K.grouped_linear(both[:12], w, off, out=both[6:]))
+    refused(lambda: K.grouped_linear(a, w, off, None, "none", both[:12], out=both[6:]))
+    refused(lambda: K.grouped_linear(a, w, off, None, "relu", r, preact=r))
+    refused(lambda: K.grouped_linear(a, w, off, None, "relu", out=r, preact=r))
+    refused(lambda: K.grouped_linear(a, w, off, None, "relu", preact=a))
+    neighbours = n(24, 16)
+    out = K.grouped_linear(a, w, off, None, "relu", out=neighbours[:12], preact=neighbours[12:])
+    assert torch.equal(out, S.grouped_linear(a, w, off, activation="relu"))
