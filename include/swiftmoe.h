@@ -161,7 +161,7 @@ SMOE_API int smoe_combine(const void* y, int dtype, const int32_t* slot_row, con
  *
  * smoe_sort_rows: rows[slot_row[t,j],:] = w[t,j] * x[t,:]; every other row of the
  * rows_cap rows becomes zero: those from expert_offsets[E] on and, when row_token is
- * given (plans with row_align > 1), the alignment padding.  With dw != NULL (needs w) also
+ * given (plans with row_align > 1; rows_cap entries), the alignment padding.  With dw != NULL (needs w) also
  * dw[t,j] = <x[t,:], y[slot_row[t,j],:]> (0 for slots without a row): called with x = the
  * gradient of smoe_unsort_rows' output and y = its rows, this is that call's gradient.  With
  * rows == NULL (expert_offsets and row_token unused) it is dw alone, in either direction.

@@ -189,6 +189,11 @@ def sort_rows(x: torch.Tensor, plan: dict, w: Optional[torch.Tensor] = None, *, 
     dt = L.dtype_code(x.dtype)
     rows = None if only_dw else torch.empty((rows_cap, d), dtype=x.dtype, device=dev)
     dw = torch.empty((T, k), dtype=torch.float32, device=dev) if y is not None else None
+    if row_token is not None and rows_cap > row_token.numel():
+        # row_token is read up to the offsets' total, which only rows_cap bounds: the plan's rows
+        # by the library, those behind them here
+        rows[row_token.numel():].zero_()
+        rows_cap = row_token.numel()
     with _on(dev):
         L.check(L.load().smoe_sort_rows(x.data_ptr(), dt, slot_row.data_ptr(), L.ptr(w), T, k, d, L.ptr(row_token),
                                         L.ptr(offsets), 1 if only_dw else offsets.numel() - 1, rows_cap, L.ptr(rows),

@@ -303,6 +303,23 @@ def test_grouped_linear_keeps_what_its_gradients_need(S, needs):
     assert grad.shape == leaf.shape
 
 
+@pytest.mark.parametrize("total", [40, 1 << 30])
+def test_offsets_past_the_plan_read_nothing_behind_it(S, K, total):
+    """Rows of a larger tensor than the plan's, and a plan whose total says they are its own:
+    its rows as they should be, the ones behind it zeros."""
+    x, _, _, _, plan = routed(S, align=8)
+    cap, x = plan["rows_cap"], x.detach()
+    want = K.sort_rows(x, plan)
+    got = K.sort_rows(x, plan, rows_cap=cap + 500)
+    assert torch.equal(got[:cap], want) and not got[cap:].any()
+    assert plan["row_token"].numel() == cap
+    total_ = int(plan["offsets"][-1])
+    plan["row_token"][total_:] = -1
+    plan["offsets"][-1] = cap + total
+    got = K.sort_rows(x, plan, rows_cap=cap + 500)
+    assert torch.equal(got[:cap], want) and not got[cap:].any()
+
+
 # ----------------------------------------------------------------------------- refusals
 def test_sizes_past_32_bits(S):
     from swiftmoe_b200._lib import SwiftMoEError
