@@ -685,8 +685,9 @@ int linear_gemm_t(const void* A, const void* B, void* C, const int32_t* offsets,
 }
 
 // Raster band (m-tiles) of the weight gradients.  16384 rows, 8 groups, bands of 1 (n fastest) /
-// 8 / 32 / 64 m-tiles: 1.53 / 1.54 / 1.51 / 1.53 ms for 14336 x 4096 weights, 1.75-1.85 / 1.71-1.76
-// / 1.68-1.71 / 1.67-1.72 for 4096 x 14336; 2.0 / 1.8 / 1.7-1.8 / 1.8 for 8192 rows, 28672 x 4096.
+// 8 / 32 / 64 m-tiles: 1.75-1.85 / 1.71-1.76 / 1.68-1.71 / 1.67-1.72 ms for 4096 x 14336 weights;
+// 1.53 / 1.54 / 1.51 / 1.53 for 14336 x 4096, which is no difference; 2.0 / 1.8 / 1.7-1.8 / 1.8
+// for 8192 rows, 28672 x 4096.
 constexpr int kWgradBand = 32;
 
 // K slices of a weight gradient's tiles, for evenly filled groups.

@@ -5,13 +5,15 @@
 // issuing tcgen05.mma (128 x 256 x 16) into one of two TMEM accumulators, epilogue warps
 // draining the other, every wait bounded -- with what these layers need besides:
 //   * bias, activation, residual and pre-activations in the epilogue, by eight warps (two per
-//     TMEM lane quarter, each 128 of the 256 columns): an exact GELU over a tile costs four
-//     warps about 19k cycles, more than the products of a tile up to K = 2400;
+//     TMEM lane quarter, each 128 of the 256 columns).  A tile's epilogue takes them 4.3 us
+//     without an activation, 6.3 with SiLU, 7.3 with the exact GELU (16384 x 14336 outputs, K = 64),
+//     and 7.3 us are the products of a tile for K = 1700: four warps would take twice as long;
 //   * weights in either layout: [N, K] K-major, or [K, N] as an MN-major operand (the input
 //     gradient reads the weights as they are, no transposed copy);
 //   * two producer warps, which share the four to six boxes of an MN-major stage (a stage's
-//     MMAs take 512 cycles; input gradient of 16384 x 14336 x 4096: 1.39 to 1.50 ms with one
-//     warp, 1.38 to 1.42 with two, 1.70 with one that also leaves out boxes past N);
+//     MMAs take 512 cycles).  Input gradient of 16384 x 14336 x 4096: 1.38 to 1.42 ms; with one
+//     warp 1.39 to 1.50, so what it gains is the slow end; 1.70 with one that also leaves out
+//     boxes past N;
 //   * launches of few tiles cut along K, the partial tiles summed by a second launch over the
 //     whole GPU (split_units below);
 //   * weight-gradient groups that start at any row, 16-bit gradients.
@@ -181,7 +183,10 @@ __device__ __forceinline__ void load_acc64(uint32_t taddr, uint32_t (&v)[64]) {
 
 // This warp's 32 accumulator rows (first row `row`, nrows valid), columns col0 .. col0 + 127
 // below N: plus bias, pre-activation out, activation, plus residual, out.  Bias (the same
-// pieces for every lane) and residual are requested before the accumulator is read.
+// pieces for every lane) and residual are requested before the accumulator is read.  The
+// output is rounded once, from fp32; the pre-activation is kept for the gradient in 16 bits
+// (fp32 would double its 0.47 GB out and back in for 16384 x 14336), which puts an error of
+// half a step of z into the argument of act'.
 template <typename T>
 __device__ __forceinline__ void epilogue_tile(uint32_t tbase, int g, int row, int nrows, int col0, int N,
                                               T* __restrict__ C, const LinearEpi& lin, unsigned char* stage, int lane) {
@@ -522,7 +527,9 @@ __global__ void __launch_bounds__(256) linear_sum_kernel(T* __restrict__ C, cons
 // add up across the warp.  The pieces of the next step -- of the same column or the warp's
 // next one -- are requested before the current ones are used, so a column's reduction does
 // not leave the memory idle (one token's two of eight experts, 14336 x 4096: 50.4 us without,
-// 38.2 with it; the 235 MB take 36).
+// 38 to 41 with it; the 235 MB take 36.  Both rows in one expert: 35, where its 117 MB take
+// 18 -- two multiplications per weight from shared memory set the time).  The choice is by
+// rows_cap, which the host knows; how many of a larger buffer's rows are in groups, it does not.
 constexpr int GEMV_ROWS = 2, GEMV_U = 8, GEMV_THREADS = 256;
 
 template <typename T>

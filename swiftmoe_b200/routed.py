@@ -157,8 +157,11 @@ def grouped_linear(a: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     a [R, K] and weight [G, N, K] bf16 / fp16, K and N multiples of 8; offsets [G+1] int32 on
     the device (``plan["offsets"]``; groups may start anywhere); bias [G, N] in a's dtype or
     fp32; activation "none", "relu", "gelu" (exact), "gelu_tanh" or "silu"; residual [R, N].
-    fp32 accumulation, one rounding.  Differentiable in a, weight, bias and residual; the
-    backward keeps the pre-activations, rounded to a's dtype, from the forward."""
+    fp32 accumulation, one rounding; an activation's own relative error is 2^-19, at |z| = 10 up
+    to 2^-15 (that of an exponential's argument).  Differentiable in a, weight, bias and
+    residual.  With an activation two things are rounded to a's dtype on the way back: the
+    pre-activations that the forward keeps, and the gradient dz in front of them, which da
+    and dweight are products of (dbias sums it unrounded)."""
     K._act_code(activation)
     if _grads_wanted(a, weight, bias, residual):
         return _GroupedLinear.apply(a, weight, bias, residual, offsets, activation)
