@@ -1235,6 +1235,14 @@ int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const fl
 #undef SMOE_ROWS_DISPATCH
 #undef SMOE_ROWS_CASE
 
+namespace {
+// Two buffers (null: absent) share memory.
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+  return a && b && p < q + b_bytes && q < p + a_bytes;
+}
+}  // namespace
+
 size_t smoe_grouped_linear_workspace_size(int64_t rows_cap, int N, int K, int G, int w_layout) {
   if (rows_cap < 1 || N < 1 || K < 1 || G < 1 || (w_layout == SMOE_W_NK && linear_gemv_rows(rows_cap, K))) return 0;
   return linear_split_plan(rows_cap, N, K, G).bytes();
@@ -1254,6 +1262,13 @@ int smoe_grouped_linear(const void* A, const void* W, int w_layout, const void* 
   if (!A || !W || !C || !offsets) return SMOE_ERR_INVALID;
   for (const void* p : {A, W, bias, residual, (const void*)preact, (const void*)C, (const void*)workspace})
     if (!aligned16(p)) return SMOE_ERR_UNSUPPORTED;
+  const size_t a_bytes = (size_t)rows_cap * K * 2, c_bytes = (size_t)rows_cap * N * 2, w_bytes = (size_t)G * N * K * 2;
+  if (overlap(C, c_bytes, A, a_bytes) || overlap(C, c_bytes, W, w_bytes) ||
+      (C != residual && overlap(C, c_bytes, residual, c_bytes)))
+    return SMOE_ERR_INVALID;
+  if (overlap(preact, c_bytes, A, a_bytes) || overlap(preact, c_bytes, W, w_bytes) ||
+      overlap(preact, c_bytes, residual, c_bytes) || overlap(preact, c_bytes, C, c_bytes))
+    return SMOE_ERR_INVALID;
   LinearEpi lin;
   lin.bias = bias;
   lin.bias_f32 = bias && bias_dtype == SMOE_F32;

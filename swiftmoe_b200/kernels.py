@@ -281,12 +281,6 @@ def _linear_dtype(t: torch.Tensor) -> int:
     return L.dtype_code(t.dtype)
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Two contiguous tensors share memory."""
-    p, q = a.data_ptr(), b.data_ptr()
-    return p < q + b.numel() * b.element_size() and q < p + a.numel() * a.element_size()
-
-
 def _group_offsets(offsets: torch.Tensor, G: int):
     if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() != G + 1 or G < 1:
         raise L.SwiftMoEError(f"offsets must be int32 [{max(G, 1) + 1}], got {offsets.dtype} {tuple(offsets.shape)}")
@@ -316,11 +310,6 @@ def grouped_linear(A: torch.Tensor, W: torch.Tensor, offsets: torch.Tensor, bias
     for name, t in (("residual", residual), ("preact", preact), ("out", out)):
         if t is not None and (t.dtype != A.dtype or t.shape != (rows_cap, N)):
             raise L.SwiftMoEError(f"{name} must be {A.dtype} [{rows_cap}, {N}], got {t.dtype} {tuple(t.shape)}")
-    if out is not None and (_overlap(out, A) or _overlap(out, W) or (
-            residual is not None and out.data_ptr() != residual.data_ptr() and _overlap(out, residual))):
-        raise L.SwiftMoEError("out may be the residual, but must not overlap A, W or a part of the residual")
-    if preact is not None and any(t is not None and _overlap(preact, t) for t in (A, W, residual, out)):
-        raise L.SwiftMoEError("preact must not overlap A, W, the residual or out")
     fill = out is None
     if out is None:
         out = torch.empty((rows_cap, N), dtype=A.dtype, device=dev)

@@ -42,7 +42,7 @@ def _grads_wanted(*ts) -> bool:
 
 def _sizes(plan: dict) -> dict:
     """What a backward needs of a plan besides tensors, as it is now: the dict is the caller's."""
-    return {n: plan.get(n) for n in ("T", "k", "rows_cap", "row_align")}
+    return {"T": plan["T"], "k": plan["k"], "rows_cap": plan["rows_cap"], "row_align": plan.get("row_align")}
 
 
 class _SortTokens(torch.autograd.Function):
@@ -71,8 +71,9 @@ class _UnsortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, w, residual, plan):
         ctx.sizes, ctx.rows_cap = _sizes(plan), rows.shape[0]
-        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, w, plan["slot_row"], plan["offsets"],
-                              plan["row_token"] if plan.get("row_align") != 1 else None)
+        need_rows, need_w = ctx.needs_input_grad[:2]
+        ctx.save_for_backward(rows if need_w else None, w, plan["slot_row"], plan["offsets"] if need_rows else None,
+                              plan["row_token"] if need_rows and plan.get("row_align") != 1 else None)
         return K.unsort_rows(rows, plan, w, residual)
 
     @staticmethod
