@@ -6,7 +6,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <initializer_list>
@@ -746,20 +745,28 @@ cudaError_t launch_act_bwd(const void* dout, const void* z, void* dz, int act, c
 
 // ------------------------------------------------------------------ tokens <-> rows
 // One warp per token, or the eight warps of a block for few tokens with long rows: below
-// `per_sm` tokens per SM.  Where the two cross, from a sweep of 16 to 6000 tokens over rows of
-// 128 to 1024 16-byte pieces and 1 to 8 slots: sort near 16 tokens per SM whatever the rows (one
-// warp / eight, 4096 x 2 bf16: 5.0 / 4.7 us for 1000 tokens, 7.0 / 6.8 for 1776, 14.3 / 17.2
-// for 4000), with dw near 7 (7.1 / 5.6 for 600, 7.3 / 7.0 for 1000, 9.7 / 13.0 for 2000).
-// unsort's single warp waits for its k rows in turn, but eight warps a token reach less of the
-// memory's rate the more slots there are: it crosses at 3 to 7 tokens per SM for 32 pieces per
-// slot (1024 x 4 bf16: 3.6 / 2.8 for 300, 4.2 / 6.1 for 1400), at 18 for 256 (4096 x 2 bf16: 7.8 /
-// 7.3 for 2000, 14.9 / 16.8 for 4000) and above 30 for 1024 -- about the root of their number,
-// three quarters of it with dw.  Rows of less than half a block's pieces keep one warp: 6.6
-// (sort with dw) and 3.5 against 12.9 and 8.8 for 4000 x 2 rows of 64.
+// `per_sm` tokens per SM.  Eight warps share a row's steps but reach less of the memory's rate.
+// Where the two cross, over 16 to 6000 tokens of 17 kinds of rows (1024 to 8192 columns of 2 and
+// 4 bytes, loads of 2 to 16 bytes, 1 to 8 slots):
+//   unsort waits for its k rows in turn, so its steps decide: at 3 to 5 tokens per SM with two
+//   steps of a warp over the row, 6 to 12 with four, 10 to 27 with eight, above 40 with 16 (4096 x 2
+//   bf16, one warp / eight: 6.4 / 4.8 us for 1000 tokens, 7.8 / 7.3 for 2000, 14.9 / 16.8 for 4000;
+//   1024 x 4: 3.6 / 2.8 for 300, 4.2 / 6.1 for 1400); with dw a step is twice as long, 2 to 5 / 4
+//   to 12 / 4 to 16 / 13 to 27 with one / two / four / eight steps;
+//   sort sends all it stores on its way at once: pieces stored per token, 4 to 6 tokens per SM
+//   for 512 of 16 bytes, 10 to 18 for 1024, 20 and more beyond (4096 x 2 bf16: 5.0 / 4.7 for 1000,
+//   7.0 / 6.8 for 1776, 14.3 / 17.2 for 4000), with dw 7 at most (7.3 / 7.0 for 1000, 9.7 / 13.0
+//   for 2000).
+// Rows of less than half a block's pieces keep one warp: 6.6 (sort with dw) and 3.5 against 12.9
+// and 8.8 for 4000 x 2 rows of 64.
 int token_warps(int T, int64_t pieces, double per_sm) { return pieces >= 128 && T < per_sm * device_sms() ? 8 : 1; }
-double sort_per_sm(bool dw) { return dw ? 6 : 12; }
-double unsort_per_sm(int64_t row_bytes, int k, bool dw) {
-  return std::min(32.0, std::sqrt((double)row_bytes / (16 * k))) * (dw ? 0.75 : 1);
+double sort_per_sm(int64_t pieces, int bytes, int k, bool dw) {
+  const double stored = (double)pieces * k / (bytes == 16 ? 1 : 2);  // (narrow pieces: twice as many in flight)
+  return std::min(dw ? 7.0 : 16.0, std::max(4.0, stored / 100));
+}
+double unsort_per_sm(int64_t pieces, int bytes, bool dw) {
+  const int step = 32 * (dw ? 4 : 2) * (bytes == 16 ? 1 : bytes == 8 ? 2 : 4);  // pieces, as in the kernel
+  return std::min(32.0, 2.0 * pieces / step);
 }
 // waves: blocks per SM at most.  sort hands its tokens to 64 (222 us with 8, 193 with 64 for
 // 32768 x 8 fp16 rows of 2048: short blocks even out the end), unsort keeps 8 resident ones.
@@ -1188,7 +1195,8 @@ int smoe_sort_rows(const void* x, int dtype, const int32_t* slot_row, const floa
   if ((rows_cap > 0 && !rows && !dw) || (!expert_offsets && (rows || !dw)) || (T > 0 && (!x || !slot_row)) ||
       (dw && (!w || (rows_cap > 0 && !y))))
     return SMOE_ERR_INVALID;
-  const int vec = row_vec(es, d, {x, rows, dw ? y : nullptr}), wpt = token_warps(T, d / vec, sort_per_sm(dw != nullptr));
+  const int vec = row_vec(es, d, {x, rows, dw ? y : nullptr});
+  const int wpt = token_warps(T, d / vec, sort_per_sm(d / vec, vec * es, k, dw != nullptr));
   cudaStream_t st = (cudaStream_t)stream;
 #define SMOE_ROWS_LAUNCH(TY, VV, WW) \
   (launch_sort_rows<TY, VV, WW>(x, slot_row, w, T, k, d, row_token, expert_offsets, E, rows_cap, rows, y, dw, st))
@@ -1223,7 +1231,7 @@ int smoe_unsort_rows(const void* y, int dtype, const int32_t* slot_row, const fl
   if (T == 0) return SMOE_OK;
   if (!slot_row || !out || (rows_cap > 0 && !y) || (dw && (!w || !x))) return SMOE_ERR_INVALID;
   const int vec = row_vec(es, d, {y, out, residual, dw ? x : nullptr});
-  const int wpt = token_warps(T, d / vec, unsort_per_sm((int64_t)d * es, k, dw != nullptr));
+  const int wpt = token_warps(T, d / vec, unsort_per_sm(d / vec, vec * es, dw != nullptr));
   cudaStream_t st = (cudaStream_t)stream;
 #define SMOE_ROWS_LAUNCH(TY, VV, WW) \
   (launch_unsort_rows<TY, VV, WW>(y, slot_row, w, T, k, d, rows_cap, residual, out, x, dw, st))
