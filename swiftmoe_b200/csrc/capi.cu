@@ -766,7 +766,7 @@ double sort_per_sm(int64_t pieces, int bytes, int k, bool dw) {
 }
 double unsort_per_sm(int64_t pieces, int bytes, bool dw) {
   const int step = 32 * (dw ? 4 : 2) * (bytes == 16 ? 1 : bytes == 8 ? 2 : 4);  // pieces, as in the kernel
-  return std::min(32.0, 2.0 * pieces / step);
+  return std::min(32.0, 2.5 * pieces / step);
 }
 // waves: blocks per SM at most.  sort hands its tokens to 64 (222 us with 8, 193 with 64 for
 // 32768 x 8 fp16 rows of 2048: short blocks even out the end), unsort keeps 8 resident ones.
