@@ -173,12 +173,12 @@ __device__ __forceinline__ void add_bias(const LinearEpi& lin, int64_t at, float
 // dz = dout * act'(z) for the rows of the groups, and the bias gradient db[g] = the sum
 // of dz over the group's rows, from the unrounded fp32 products.  dz itself is rounded to the
 // layer's type, as an operand of the 16-bit tensor-core products that make dA and dW of it.
-// Memory-bound: dout and z read once, dz written once.  A block owns 256 columns (a lane 8 of them) of `slice`
-// consecutive rows, its eight warps every eighth row; it walks the groups its rows belong
-// to and writes one partial row of column sums per group to part[s + g], which is a
-// different row for every (slice s, group g) pair that has rows, since both only grow
-// along the rows.  bias_grad_reduce_kernel adds a group's partials in slice order, so no
-// result depends on the order in which blocks run.
+// Memory-bound: dout and z read once, dz written once.  A block owns 256 columns (a lane 8 of
+// them) of `slice` consecutive rows, its eight warps every eighth row; it walks the groups its
+// rows belong to and writes one partial row of column sums per group to part[s + g], which is
+// a different row for every (slice s, group g) pair that has rows, since both only grow along
+// the rows.  bias_grad_reduce_kernel adds a group's partials in slice order, so no result
+// depends on the order in which blocks run.
 constexpr int kActCols = 256, kActGroups = 1024;
 
 template <typename T, int ACT, bool BIAS>
